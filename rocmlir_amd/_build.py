@@ -109,14 +109,35 @@ def attention_kernels():
     return out
 
 
+TOKEN_TYPES = {0: "f32", 1: "f16", 2: "bf16", 3: "i8"}
+
+
+def token_kernels(type_code):
+    """[(kernel name, macro invocation)] of the products of token rows (csrc/token_gemm.h) for one operand type."""
+    t = TOKEN_TYPES[type_code]
+    out = []
+    for tile in ("_256x256", "_128x128", "_64x64"):
+        dims = "%d, %d, %d, %d" % TILES[tile]
+        out.append(("rock_token_gemm_%s%s_fast" % (t, tile), "RK_TOKEN_GEMM_DL(%s_fast, %s, %s)" % (tile, dims, ROWS)))
+        out.append(("rock_token_gemm_%s%s_fast_nn" % (t, tile), "RK_TOKEN_GEMM_DL(%s_fast_nn, %s, %s)" % (tile, dims, COLS)))
+        if t != "i8":
+            out.append(("rock_token_gemm_bwd_weight_%s%s" % (t, tile), "RK_TOKEN_WEIGHT_DL(%s, %s)" % (tile, dims)))
+    out.append(("rock_token_gemm_%s_64x64_generic" % t, "RK_TOKEN_GEMM(_64x64_generic, 64, 64, 2, 2)"))
+    if t != "i8":
+        out.append(("rock_token_gemm_bwd_weight_%s_64x64_generic" % t, "RK_TOKEN_WEIGHT(_64x64_generic, 64, 64, 2, 2)"))
+    return out
+
+
 # translation units of the host side (csrc/<unit>.cpp)
-HOST_UNITS = ["rock_options", "plan_gemm", "plan_relayout", "plan_conv", "plan_conv_bwd_data", "plan_conv_bwd_weight",
+HOST_UNITS = ["rock_options", "plan_gemm", "plan_tokens", "plan_relayout", "plan_conv", "plan_conv_bwd_data", "plan_conv_bwd_weight",
               "plan_conv3d", "plan_attention", "rock_handle", "rock_launch", "miir_api", "bench_api"]
 
 # kernels of csrc/relayout_kernels.hip in file order (-DROCK_KERNEL=<position>)
 RELAYOUT_KERNELS = ["rock_relayout_b1", "rock_relayout_b2", "rock_relayout_b4", "rock_fill_zero",
                     "rock_reduce_splits", "rock_softmax_rows", "rock_relayout_pair_b1", "rock_relayout_pair_b2",
                     "rock_relayout_pair_b4", "rock_fold_depth"]
+# kernels of csrc/quantize_tokens.hip in file order
+QUANTIZE_KERNELS = ["rock_quantize_tokens_f32", "rock_quantize_tokens_f16", "rock_quantize_tokens_bf16"]
 # kernels of csrc/probe_kernels.hip by operand-type code (-DROCK_KERNEL=<code>)
 PROBE_KERNELS = {0: "rock_probe_mfma_f32", 1: "rock_probe_mfma_f16", 2: "rock_probe_mfma_bf16",
                  3: "rock_probe_mfma_i8", 4: "rock_probe_mfma_fp8"}
@@ -142,6 +163,13 @@ def device_jobs():
     for name, macro in attention_kernels():
         text = "// generated by rocmlir_amd/_build.py\n#include \"attention_kernels.h\"\n%s\n" % macro
         jobs.append((name, os.path.join(GEN, name + ".hip"), text, []))
+    for code, t in TOKEN_TYPES.items():
+        for name, macro in token_kernels(code):
+            text = ("// generated by rocmlir_amd/_build.py\n#define ROCK_DT %d\n#define ROCK_DTNAME %s\n"
+                    "#include \"token_gemm.h\"\n%s\n" % (code, t, macro))
+            jobs.append((name, os.path.join(GEN, name + ".hip"), text, []))
+    for i, name in enumerate(QUANTIZE_KERNELS):
+        jobs.append((name, os.path.join(CSRC, "quantize_tokens.hip"), None, ["-DROCK_KERNEL=%d" % i]))
     for i, name in enumerate(RELAYOUT_KERNELS):
         jobs.append((name, os.path.join(CSRC, "relayout_kernels.hip"), None, ["-DROCK_KERNEL=%d" % i]))
     for code, name in PROBE_KERNELS.items():

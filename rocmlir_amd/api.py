@@ -343,6 +343,7 @@ class RockProgram:
 
     def __init__(self, options):
         self.options = options
+        self.lock = threading.Lock()   # a handle must not be used from two threads at once
         self._build(options)
 
     def _build(self, options):
@@ -357,7 +358,7 @@ class RockProgram:
         """The contraction kernel: the last GEMM, convolution or attention kernel of the list (conversion
         kernels may run in front of it, the reduction of split partial sums behind it)."""
         for k in reversed(self.kernels):
-            if k.kernel_name.startswith(("rock_gemm_", "rock_conv_", "rock_attention_")):
+            if k.kernel_name.startswith(("rock_gemm_", "rock_conv_", "rock_attention_", "rock_token_gemm_")):
                 return k
         return self.kernels[-1]
 
@@ -515,7 +516,8 @@ def gemm(a, b, *, transA=False, transB=False, transC=False, out_dtype=None,
          scale=None, zero_point=0, bias=None, relu=False, quant_scale=None,
          out_zero_point=0, activation=None, clip=None, residual=None,
          residual_op="add", out=None, perf_config=None, stream=None,
-         info=None, split_k=True, layout_conversion=True, accumulate=False):
+         info=None, split_k=True, layout_conversion=True, accumulate=False,
+         token_scale=None):
     """C = epilogue(A x B) with the reference's storage conventions
     (rocmlir-gen.cpp:2058-2080): a is [G,M,K] ([G,K,M] if transA), b is
     [G,K,N] ([G,N,K] if transB), result [G,M,N] ([G,N,M] if transC).
@@ -532,8 +534,20 @@ def gemm(a, b, *, transA=False, transB=False, transC=False, out_dtype=None,
     into padded ones unless `layout_conversion` is False; a long reduction
     over few output tiles is split over blocks unless `split_k` is False).
     `accumulate=True` (rocmlir-gen's -store-method atomic_add) adds the
-    result into `out` instead of overwriting it."""
+    result into `out` instead of overwriting it.
+
+    `token_scale` (int8 operands, G = 1): a float32 tensor with one value per
+    row of the result, as quantize_tokens() returns it; the result is
+    (sum - zero_point) * scale[n] * token_scale[m] (+ bias, then relu or clip)
+    in `out_dtype` f16 (the default), bf16 or f32.  K up to 131071; no transA,
+    transC, residual, requantisation or accumulation beside it."""
     import torch
+    if token_scale is not None:
+        if transA or transC or accumulate or residual is not None or quant_scale is not None or _is_tensor(zero_point) \
+                or _is_tensor(out_zero_point) or out_zero_point:
+            raise RockError("gemm: token_scale takes scale, a scalar zero_point, bias, relu and clip only")
+        return _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, activation, clip, out,
+                                  perf_config, stream, info, token_scale)
     if accumulate and (out is None or residual is not None):
         raise RockError("gemm: accumulate=True adds into `out` and takes no residual")
     a3 = a if a.dim() == 3 else a.unsqueeze(0)
@@ -878,3 +892,250 @@ def conv2d_bwd_weight(inp, dout, *, fil_layout, in_layout, out_layout, batchsize
                           device=dout.device)
     prog.launch(out, inp.contiguous(), dout.contiguous(), None, stream=stream)
     return out
+
+
+# ---------------------------------------------------------------------------
+# operators over the token rows of a language model (csrc/plan_tokens.cpp)
+# ---------------------------------------------------------------------------
+_token_plans = {}
+
+
+def _token_plan(*key):
+    """The plan of a problem given as (operation, type, (option, value), ...); `key` is its cache entry."""
+    p = _token_plans.get(key)
+    if p is None:
+        opts = "-operation %s -arch gfx950 -t %s" % key[:2] + "".join(" -%s %s" % kv for kv in key[2:] if kv[1] is not None)
+        p = RockProgram(opts)
+        if len(_token_plans) >= 4096:   # token counts change from call to call
+            _token_plans.clear()
+        _token_plans[key] = p
+    return p
+
+
+def _dense(t):
+    """`t` as the kernels address it: contiguous, from a 16-byte boundary on."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _TokenCall:
+    """Where the tensors' work runs: their device is made the current one, `stream` (default: the device's current
+    stream) torch's current stream, so that copies and results made on the way are ordered with the kernels."""
+
+    def __init__(self, name, stream, **tensors):
+        self.name = name
+        self.device = next(t.device for t in tensors.values() if t is not None)
+        for what, t in tensors.items():
+            if t is not None and t.device != self.device:
+                raise RockError("%s: %s is on %s, the other tensors on %s" % (name, what, t.device, self.device))
+        self._contexts = []
+        if self.device.type == "cuda":
+            import torch
+            if self.device.index != torch.cuda.current_device():
+                self._contexts.append(torch.cuda.device(self.device))
+            if stream is not None:
+                if not isinstance(stream, torch.cuda.Stream):
+                    stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=self.device)
+                if stream.device != self.device:
+                    raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, self.device))
+                self._contexts.append(torch.cuda.stream(stream))
+
+    def __enter__(self):
+        for c in self._contexts:
+            c.__enter__()
+        return self
+
+    def __exit__(self, *exc):
+        for c in reversed(self._contexts):
+            c.__exit__(*exc)
+
+    def result(self, out, shape, dtype):
+        """`out` checked, or a new tensor."""
+        import torch
+        if out is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != self.device:
+            raise RockError("%s: out must be %s of %s on %s" % (self.name, tuple(shape), dtype, self.device))
+        if not out.is_contiguous() or out.data_ptr() % 16:
+            raise RockError("%s: out must be contiguous and start on a 16-byte boundary" % self.name)
+        return out
+
+    def launch(self, prog, info, *tensors):
+        if info is not None:
+            info["kernels"] = [k.kernel_name for k in prog.kernels]
+            info["kernel_name"] = prog.kernel_name
+            info["perf_config"] = prog.perf_config
+        with prog.lock:
+            for k in prog.kernels:
+                k.launch(*tensors)
+
+
+def _check_scale_vector(name, what, t, count):
+    import torch
+    if not _is_tensor(t) or t.dtype != torch.float32 or t.numel() != count:
+        raise RockError("%s: %s must hold %d float32 elements" % (name, what, count))
+    return _dense(t)
+
+
+def quantize_tokens(x, *, out=None, scale_out=None, stream=None, info=None):
+    """Quantises every row of x [..., K] (f16, bf16 or f32) to int8 with a scale of its own, the operands of gemm()
+    and grouped_gemm() with `token_scale`: scale = max |x| / 127, q = roundeven(127 x / max |x|).  A row of zeros has
+    scale 0 and q = 0; a row that holds an infinity or a NaN has scale NaN and q = 0, so that products of this row,
+    and of no other, are NaN.  Returns (q [..., K] int8, scale [...] float32), written into `out` and `scale_out`
+    where given."""
+    import torch
+    if x.dim() < 1 or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise RockError("quantize_tokens: x is [..., K] of f16, bf16 or f32")
+    cols = x.shape[-1]
+    with _TokenCall("quantize_tokens", stream, x=x, out=out, scale_out=scale_out) as call:
+        q = call.result(out, x.shape, torch.int8)
+        s = call.result(scale_out, x.shape[:-1], torch.float32)
+        if x.numel() == 0:
+            if s.numel():       # rows without elements: their largest magnitude is 0
+                s.zero_()
+            return q, s
+        prog = _token_plan("quantize_tokens", _dtype_name(x.dtype), ("m", x.numel() // cols), ("k", cols))
+        call.launch(prog, info, _dense(x), q, s)
+    return q, s
+
+
+def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, activation, clip, out, perf_config, stream,
+                       info, token_scale):
+    """gemm() with a scale for each row of the result."""
+    import torch
+    name = "gemm with token_scale"
+    if a.dtype != torch.int8 or b.dtype != torch.int8:
+        raise RockError("%s: int8 operands" % name)
+    if a.dim() not in (2, 3) or b.dim() not in (2, 3) or (a.dim() == 3 and a.shape[0] != 1) or (b.dim() == 3 and b.shape[0] != 1):
+        raise RockError("%s: one batch entry" % name)
+    M, K = a.shape[-2:]
+    Kb, N = (b.shape[-1], b.shape[-2]) if transB else (b.shape[-2], b.shape[-1])
+    if Kb != K:
+        raise RockError("%s: operand shapes do not match" % name)
+    if activation not in (None, "relu", "clip") or (activation == "clip" and clip is None):
+        raise RockError("%s: activations relu and clip only" % name)
+    out_dtype = out_dtype or "f16"
+    if out_dtype not in ("f16", "bf16", "f32"):
+        raise RockError("%s: out_dtype f16, bf16 or f32" % name)
+    vector = _is_tensor(scale)
+    with _TokenCall(name, stream, a=a, b=b, token_scale=token_scale, scale=scale if vector else None, bias=bias, out=out) as call:
+        ts = _check_scale_vector(name, "token_scale", token_scale, M)
+        cs = _check_scale_vector(name, "scale", scale, N) if vector else None
+        bv = None if bias is None else _check_scale_vector(name, "bias", bias, N)
+        res = call.result(out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype))
+        if M == 0:
+            return res
+        prog = _token_plan("gemm", "i8", ("m", M), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
+                           ("out_datatype", out_dtype), ("token_scale_vector", "true"),
+                           ("scale_vector", "true" if vector else None),
+                           ("scale", None if vector or scale is None else "%.9g" % scale),
+                           ("zero_point", zero_point or None), ("bias", None if bias is None else "true"),
+                           ("activation", "clip" if clip is not None else "relu" if relu else activation),
+                           ("clip_min", None if clip is None else "%.9g" % clip[0]),
+                           ("clip_max", None if clip is None else "%.9g" % clip[1]), ("perf_config", perf_config))
+        call.launch(prog, info, _dense(a), _dense(b), res, bv, ts, *([cs] if vector else []))
+    return res
+
+
+def _grouped(name, rows, w, offsets, transB, cols_of_rows):
+    """(groups, rows, N, K) of a grouped product, its operands checked; `cols_of_rows`: what `rows` holds per row."""
+    import torch
+    if w.dim() != 3 or rows.dim() != 2 or rows.dtype != w.dtype:
+        raise RockError("%s: rows [T, .] and weights [E, ., .] of one type" % name)
+    E = w.shape[0]
+    N, K = (w.shape[1], w.shape[2]) if transB else (w.shape[2], w.shape[1])
+    if rows.shape[1] != (K if cols_of_rows == "K" else N):
+        raise RockError("%s: operand shapes do not match" % name)
+    _check_offsets(name, offsets, E)
+    return E, rows.shape[0], N, K
+
+
+def _check_offsets(name, offsets, E):
+    import torch
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != E + 1:
+        raise RockError("%s: offsets is int32 [E + 1], the first row of every expert and the end of the last" % name)
+    if E == 0:
+        raise RockError("%s: no experts" % name)
+
+
+def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=None, scale=None, out=None, stream=None,
+                 perf_config=None, info=None):
+    """Products grouped by expert: rows offsets[e] <= t < offsets[e + 1] of x [T, K] times w[e], w [E, K, N]
+    ([E, N, K] if transB) -> [T, N].  `offsets` is int32 [E + 1] on the GPU, never read on the host: non-decreasing
+    values within [0, T] (an offset that steps back or lies outside is taken as the furthest one before it).  Experts
+    may have no rows; rows of no expert are not written: they keep what `out` held (undefined without `out`).  f16,
+    bf16 and f32 operands give a result of their type unless `out_dtype` names another of the three; int8 operands
+    give sum * scale * token_scale as f16 (default), bf16 or f32, `token_scale` float32 [T], `scale` float32 [E, N] or
+    a number (both optional)."""
+    import torch
+    name = "grouped_gemm"
+    E, T, N, K = _grouped(name, x, w, offsets, transB, "K")
+    i8 = x.dtype == torch.int8
+    t = _dtype_name(x.dtype)
+    if t not in ("f32", "f16", "bf16", "i8"):
+        raise RockError("%s: f16, bf16, f32 or int8 operands" % name)
+    if not i8 and (token_scale is not None or scale is not None):
+        raise RockError("%s: scales go with int8 operands" % name)
+    out_dtype = out_dtype or ("f16" if i8 else t)
+    if out_dtype not in ("f16", "bf16", "f32"):
+        raise RockError("%s: out_dtype f16, bf16 or f32" % name)
+    vector = _is_tensor(scale)
+    with _TokenCall(name, stream, x=x, w=w, offsets=offsets, token_scale=token_scale, scale=scale if vector else None,
+                    out=out) as call:
+        scales = []
+        if token_scale is not None:
+            scales.append(_check_scale_vector(name, "token_scale", token_scale, T))
+        if vector:
+            scales.append(_check_scale_vector(name, "scale", scale, E * N))
+        res = call.result(out, (T, N), _torch_dtype(out_dtype))
+        if T == 0 or N == 0:
+            return res
+        prog = _token_plan("grouped_gemm", t, ("g", E), ("m", T), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
+                           ("out_datatype", out_dtype), ("token_scale_vector", None if token_scale is None else "true"),
+                           ("scale_vector", "true" if vector else None),
+                           ("scale", None if vector or scale is None else "%.9g" % scale), ("perf_config", perf_config))
+        call.launch(prog, info, _dense(x), _dense(w), res, _dense(offsets), *scales)
+    return res
+
+
+def grouped_gemm_bwd_data(dout, w, offsets, *, transB=False, out=None, stream=None, perf_config=None, info=None):
+    """Gradient of grouped_gemm() with respect to x: rows of `dout` [T, N] times the transpose of their expert's
+    weights (w and transB as given to grouped_gemm) -> [T, K] of dout's type, f16, bf16 or f32.  Rows of no expert
+    are not written."""
+    name = "grouped_gemm_bwd_data"
+    E, T, N, K = _grouped(name, dout, w, offsets, transB, "N")
+    t = _dtype_name(dout.dtype)
+    if t not in ("f32", "f16", "bf16"):
+        raise RockError("%s: f16, bf16 or f32 operands" % name)
+    with _TokenCall(name, stream, dout=dout, w=w, offsets=offsets, out=out) as call:
+        res = call.result(out, (T, K), dout.dtype)
+        if T == 0 or K == 0:
+            return res
+        prog = _token_plan(name, t, ("g", E), ("m", T), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
+                           ("perf_config", perf_config))
+        call.launch(prog, info, res, _dense(w), _dense(dout), _dense(offsets))
+    return res
+
+
+def grouped_gemm_bwd_weight(x, dout, offsets, *, transB=False, out=None, stream=None, perf_config=None, info=None):
+    """Gradient of grouped_gemm() with respect to w: for every expert the sum over its rows of x [T, K] and dout
+    [T, N] -> [E, K, N] ([E, N, K] if transB) of their type, f16, bf16 or f32, summed in f32.  An expert without rows
+    gets zeros."""
+    name = "grouped_gemm_bwd_weight"
+    if x.dim() != 2 or dout.dim() != 2 or x.shape[0] != dout.shape[0] or x.dtype != dout.dtype:
+        raise RockError("%s: x [T, K] and dout [T, N] of one type" % name)
+    E, T, K, N = offsets.shape[0] - 1, x.shape[0], x.shape[1], dout.shape[1]
+    _check_offsets(name, offsets, E)
+    t = _dtype_name(x.dtype)
+    if t not in ("f32", "f16", "bf16"):
+        raise RockError("%s: f16, bf16 or f32 operands" % name)
+    with _TokenCall(name, stream, x=x, dout=dout, offsets=offsets, out=out) as call:
+        res = call.result(out, (E, N, K) if transB else (E, K, N), x.dtype)
+        if res.numel() == 0:
+            return res
+        if T == 0:
+            return res.zero_()
+        prog = _token_plan(name, t, ("g", E), ("m", T), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
+                           ("perf_config", perf_config))
+        call.launch(prog, info, _dense(x), res, _dense(dout), _dense(offsets))
+    return res

@@ -876,7 +876,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
   if (staged_ok || cols_ok)
     __builtin_amdgcn_s_barrier(); // every wave is done reading the operand stages
 
-  dispatch_out_dtype<Tr::INT_ACC>(e.out_dtype, [&](auto od_const) __attribute__((always_inline)) {
+  dispatch_tile_dtype<Tr::INT_ACC>(p, [&](auto od_const) __attribute__((always_inline)) {
     constexpr int OD = decltype(od_const)::value;
     // plain epilogue (scale, bias, relu / clip, narrowing): unrolled over the registers
     if (cols_ok) {
@@ -891,6 +891,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
       char *wbuf = lds + wave * WBUF;
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
+        const auto rv = row_values(p, m_wave + i * 32 + lrow);
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
 #pragma unroll
@@ -898,7 +899,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
             const int nloc = j * 32 + q * 8 + lgrp * 4;
             Acc4 a4 = {acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                        acc[i][j][4 * q + 3]};
-            const v4i raw = epilogue_convert4<Tr::INT_ACC, OD>(a4, e, aux, n_wave + nloc, p.N);
+            const v4i raw = tile_convert4<Tr::INT_ACC, OD>(a4, p, rv, aux, n_wave + nloc);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               char *dst = wbuf + (nloc + r) * MP + lrow * ES;
@@ -946,6 +947,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
     const int rd_row = lane / LPR, rd_cb = (lane % LPR) * 16;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
+      const auto rv = row_values(p, m_wave + i * 32 + lrow);
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
 #pragma unroll
@@ -953,7 +955,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
           const int nloc = j * 32 + q * 8 + lgrp * 4;
           Acc4 a4 = {acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                      acc[i][j][4 * q + 3]};
-          v4i raw = epilogue_convert4<Tr::INT_ACC, OD>(a4, e, aux, n_wave + nloc, p.N);
+          v4i raw = tile_convert4<Tr::INT_ACC, OD>(a4, p, rv, aux, n_wave + nloc);
           char *dst = wbuf + lrow * PITCH + nloc * ES;
           if constexpr (ES == 4)
             *(v4i *)dst = raw;
@@ -985,10 +987,19 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
 }
 
 
+// Parameter blocks with a scale for each row of the result have an epilogue of their own (token_gemm.h).
+template <typename Params> struct HasRowScales : std::false_type {};
+template <int DT, int MI, int NI, int NWAVES, int LDS_BYTES, typename Params>
+__device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (&acc)[MI][NI], const Params &p, int g,
+                                                   void *Cptr, const void *aux, int m_wave, int n_wave, char *lds,
+                                                   int wave, int lane);
+
+// The output tile (g, m0.., n0..) by the calling block.
 template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int RB, int LDA, int LDB, bool RICH = false,
           typename Params>
-__device__ __forceinline__ void contraction_body_dl(const void *Aptr, const void *Bptr, void *Cptr,
-                                                    const void *aux, const void *res, const Params &p) {
+__device__ __forceinline__ void contraction_tile_dl(const void *Aptr, const void *Bptr, void *Cptr,
+                                                    const void *aux, const void *res, const Params &p, int g, int m0,
+                                                    int n0) {
   using Tr = MmaTraits<DT>;
   using Acc = typename Tr::Acc;
   constexpr int NW = WAVES_M * WAVES_N;
@@ -1022,10 +1033,6 @@ __device__ __forceinline__ void contraction_body_dl(const void *Aptr, const void
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave % WAVES_M, wn = wave / WAVES_M;
   const int lrow = lane & 31, lgrp = lane >> 5;
-
-  int g, tm, tn;
-  decode_block(p.tiles_m, p.tiles_n, p_batch(p), p.group_m, p.xcd_remap, g, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
 
   // Eight-wave blocks put two waves on every SIMD.  Only the upper four issue
   // loads: a burst of load instructions from all eight backs up in the
@@ -1150,8 +1157,22 @@ __device__ __forceinline__ void contraction_body_dl(const void *Aptr, const void
   char *staging = lds;
   if constexpr (KM)
     staging = wave < NW / 2 ? lds : lds_hi - (NW / 2) * WBUF;
-  dl_epilogue<DT, MI, NI, NW, kDlStages * STAGE, RICH>(acc, p, g, Cptr, aux, res, m0 + wm * WTM, n0 + wn * WTN, staging,
-                                                       wave, lane);
+  if constexpr (HasRowScales<Params>::value)
+    row_scale_epilogue<DT, MI, NI, NW, kDlStages * STAGE>(acc, p, g, Cptr, aux, m0 + wm * WTM, n0 + wn * WTN, staging,
+                                                          wave, lane);
+  else
+    dl_epilogue<DT, MI, NI, NW, kDlStages * STAGE, RICH>(acc, p, g, Cptr, aux, res, m0 + wm * WTM, n0 + wn * WTN,
+                                                         staging, wave, lane);
+}
+
+template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int RB, int LDA, int LDB, bool RICH = false,
+          typename Params>
+__device__ __forceinline__ void contraction_body_dl(const void *Aptr, const void *Bptr, void *Cptr,
+                                                    const void *aux, const void *res, const Params &p) {
+  int g, tm, tn;
+  decode_block(p.tiles_m, p.tiles_n, p_batch(p), p.group_m, p.xcd_remap, g, tm, tn);
+  contraction_tile_dl<DT, BM, BN, WAVES_M, WAVES_N, RB, LDA, LDB, RICH>(Aptr, Bptr, Cptr, aux, res, p, g, tm * BM,
+                                                                       tn * BN);
 }
 
 } // namespace rk

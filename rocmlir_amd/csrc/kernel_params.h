@@ -92,6 +92,32 @@ struct RockGemmParams {
   RockEpilogue epi;
 };
 
+// Products of token rows (token_gemm.h): rows of A times the weights of the group (expert) that the row belongs to.
+// rock_token_gemm_*(A, B, C, bias, offsets, token_scale, channel_scale, p): row m of A[M, K] that lies in
+// [offsets[e], offsets[e+1]) is multiplied with B[e] (b_gs elements apart) into row m of C; a NULL `offsets` means one
+// group of all M rows.  `gemm.M` counts all rows, `gemm.G` the groups, a_gs and c_gs are 0, tiles_m is the largest
+// number of row tiles that M rows in G groups can make.  int8 operands: C = (acc - zero_point) * s[n] * t[m] (+ bias),
+// s = channel_scale[e * N + n] or epi.scale, t = token_scale[m] or 1.
+struct RockTokenGemmParams {
+  RockGemmParams gemm;
+};
+
+// Gradient of the weights of such a product: rock_token_gemm_bwd_weight_*(A, B, C, offsets, p) adds, for every group e,
+// C[e][m, n] = sum over the rows t of [offsets[e], offsets[e+1]) of A[t, m] * B[t, n].  a_ks / b_ks are the row pitches
+// of A and B (a_ms = b_ns = 1), `gemm.K` counts all rows, `gemm.G` the groups.
+struct RockTokenWeightParams {
+  RockGemmParams gemm;
+};
+
+// rock_quantize_tokens_*(x, q, scale, p): every row of x[rows, cols] becomes int8 with one scale,
+// scale = max |x| / 127, q = roundeven(127 x / max |x|); a row of zeros has scale 0 and q = 0, a row that holds an
+// infinity or a NaN has scale NaN and q = 0.
+struct RockQuantizeParams {
+  int64_t rows;
+  int32_t cols;
+  int32_t lanes_per_row; // 64: a wave per row; 256: the block's four waves share a row
+};
+
 // Forward convolution as an implicit GEMM:
 //   M = N*Ho*Wo (output pixels), N = K_out per group, K = Y*X*C per group.
 // Strides are in elements of the respective tensor.

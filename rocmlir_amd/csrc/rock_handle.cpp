@@ -217,15 +217,32 @@ Handle *build_handle(const OptMap &given) {
     }
   }
   std::string op = str_or(o, "operation", "");
-  const int chan = channel_vector_flags(o);
+  // products of token rows (plan_tokens.cpp) take their scales as kernel pointers and describe their own arguments
+  const bool token_scaled = op == "gemm" && bool_or(o, "token_scale_vector", false);
+  const bool tokens = token_scaled || op == "quantize_tokens" || op.rfind("grouped_gemm", 0) == 0;
+  if (bool_or(o, "token_scale_vector", false) && !token_scaled && op != "grouped_gemm") {
+    set_error("token_scale_vector: gemm and grouped_gemm only");
+    return nullptr;
+  }
+  if (accumulate && tokens) {
+    set_error("store-method atomic_add: not beside token scales");
+    return nullptr;
+  }
+  const int chan = tokens ? 0 : channel_vector_flags(o);
   if (chan && !(op == "gemm" || ((op == "conv" || op == "conv2d") && !o.count("in_d") && !o.count("fil_d")))) {
     set_error("per-channel quantisation vectors: GEMM and forward 2-D convolution only");
     return nullptr;
   }
   Handle *h = nullptr;
   try {
-    if (op == "gemm")
+    if (token_scaled)
+      h = make_token_scaled_gemm(o);
+    else if (op == "gemm")
       h = make_gemm(o);
+    else if (op == "quantize_tokens")
+      h = make_quantize_tokens(o);
+    else if (op == "grouped_gemm" || op == "grouped_gemm_bwd_data" || op == "grouped_gemm_bwd_weight")
+      h = make_grouped_gemm(o);
     else if (op == "attention")
       h = make_attention(o);
     else if (op == "conv" || op == "conv2d" || op == "conv_bwd_data" || op == "conv2d_bwd_data" ||
@@ -300,6 +317,8 @@ Handle *build_handle(const OptMap &given) {
     return nullptr;
   }
   h->options = given;
+  if (tokens)
+    return h;
   if (accumulate)
     planned.erase("residual"); // C stands in for it: no such tensor in the caller's list
   describe_arguments(planned, h);
@@ -319,6 +338,8 @@ std::vector<std::string> tuning_candidates(const Handle &h, int kind) {
     for (int dmax : {64, 128})
       for (const AttnVariant &v : kAttnVariants)
         requests.push_back(attn_perf_string(v, dmax));
+  } else if (h.op == OP_TOKENS && !h.epi && h.num_pointers == 3) {
+    // quantisation: one kernel per type
   } else {
     for (const Tile &t : kFastTiles)
       requests.push_back(perf_string(t, 1));

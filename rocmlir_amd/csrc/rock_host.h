@@ -111,7 +111,7 @@ inline int64_t floor_div(int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a +
 // --------------------------------------------------------------------------
 // problems
 // --------------------------------------------------------------------------
-enum OpKind { OP_GEMM, OP_CONV, OP_ATTENTION, OP_RELAYOUT };
+enum OpKind { OP_GEMM, OP_CONV, OP_ATTENTION, OP_RELAYOUT, OP_TOKENS };
 
 struct Handle {
   OpKind op;
@@ -252,6 +252,11 @@ inline const AttnVariant kAttnVariants[] = {{"fast", 8, 1}, {"fast_bias", 8, 0},
 std::string attn_perf_string(const AttnVariant &v, int dmax);
 bool parse_attn_perf(const std::string &pc, int &dmax, int &kpack_pb, int &force_unroll);
 Handle *make_attention(const OptMap &o);
+
+// ---- token rows: plan_tokens.cpp --------------------------------------------------------------------
+Handle *make_token_scaled_gemm(const OptMap &o);
+Handle *make_grouped_gemm(const OptMap &o);
+Handle *make_quantize_tokens(const OptMap &o);
 
 // ---- handles and tuning: rock_handle.cpp ---------------------------------------------------------
 Handle *build_handle(const OptMap &o);

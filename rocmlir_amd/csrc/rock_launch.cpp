@@ -103,6 +103,8 @@ bool check_launch_args(Handle *h, void *const *pointers, int num_pointers) {
     need_aux = ap->has_bias != 0;
     aux_index = ap->has_scale_tensor ? 4 : 3;
   }
+  if (h->op == OP_TOKENS)
+    need_aux = true; // no bias slot: every pointer is a tensor
   for (int i = 0; i < num_pointers; ++i)
     if (!pointers[i] && (i != aux_index || need_aux)) {
       set_error("launch: NULL tensor pointer");

@@ -1,0 +1,427 @@
+// Products of token rows: an activation matrix whose rows belong to one group of weights or are spread over several
+// (the experts of a mixture), the gradient of such weights, and the scales per token and channel of int8 operands.
+//
+// The tiles are those of gemm_conv_dlds.h and gemm_conv_kernel.h; what is added here is
+//   * where a block's tile lies: the rows of group e are [offsets[e], offsets[e+1]), known on the device only, so the
+//     grid covers the largest number of row tiles that M rows in G groups can make and every block finds its group
+//     from the offsets by a scan over the lanes of a wave; blocks behind the last tile leave;
+//   * the epilogue that multiplies int32 sums by channel_scale[n] and token_scale[m];
+//   * the reduction over a group's rows (weight gradient), whose operands are addressed with 64-bit row positions.
+// The reference has batched products with one size for all batch entries only (RockOps.td:63-99).
+#pragma once
+#include "gemm_conv_dlds.h"
+
+namespace rk {
+
+// ---- parameter blocks of a tile -----------------------------------------------------------
+struct TokenTileParams : RockGemmParams {};
+// results are f32, f16 or bf16
+template <bool INT_ACC, typename F>
+__device__ __forceinline__ void dispatch_tile_dtype(const TokenTileParams &p, F &&f) {
+  switch (p.epi.out_dtype) {
+  case ROCK_F32: f(std::integral_constant<int, ROCK_F32>{}); break;
+  case ROCK_F16: f(std::integral_constant<int, ROCK_F16>{}); break;
+  default: f(std::integral_constant<int, ROCK_BF16>{}); break;
+  }
+}
+
+// ---- scales per token and channel -----------------------------------------------------
+struct TokenScaleParams : TokenTileParams {
+  const float *token_scale;   // of the tile's group: element m belongs to row m
+  const float *channel_scale; // element n to column n; NULL: epi.scale
+};
+struct TokenRowValues {
+  float scale;
+};
+__device__ __forceinline__ TokenRowValues row_values(const TokenScaleParams &p, int m) {
+  return {p.token_scale && m < p.M ? p.token_scale[m] : 1.0f};
+}
+// (acc - zero_point) * s[n] * t[m] + bias[n], clamped: every step one f32 operation, narrowed once at the end
+template <bool INT_ACC, int OD, bool SLOW_CALL = false, bool CHAN = false, typename Acc4>
+__device__ __forceinline__ v4i tile_convert4(const Acc4 &acc, const TokenScaleParams &p, TokenRowValues row,
+                                             const void *aux, int n0, const void * = nullptr, int64_t = 0,
+                                             int64_t = 1) {
+  const RockEpilogue &e = p.epi;
+  float s4[4] = {e.scale, e.scale, e.scale, e.scale}, b4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n0 + r < p.N) {
+      if (p.channel_scale)
+        s4[r] = p.channel_scale[n0 + r];
+      if (e.has_bias)
+        b4[r] = ((const float *)aux)[n0 + r];
+    }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    v[r] = ((float)(int)acc[r] - (float)e.zero_point) * s4[r] * row.scale;
+    if (e.has_bias)
+      v[r] = v[r] + b4[r];
+    if (e.activation)
+      v[r] = activation_fast(v[r], e);
+  }
+  return epilogue_pack4<OD>(v, e);
+}
+
+// Epilogue of the tiled kernels with these scales.  The raw sums go through the wave's LDS region, 32 rows at a time,
+// and are scaled on the way out, where a lane holds eight consecutive columns of one row: its channel scales and biases
+// are then the same for all its rows and are loaded once.  Scaled where they sit in the accumulators, every group of
+// four would load its own, behind a bounds test each, three output types over: four minutes of compilation and a hundred
+// spilled scalar registers in the 256 x 256 tile.
+template <> struct HasRowScales<TokenScaleParams> : std::true_type {};
+template <int DT, int MI, int NI, int NWAVES, int LDS_BYTES, typename Params>
+__device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (&acc)[MI][NI], const Params &p, int g,
+                                                   void *Cptr, const void *aux, int m_wave, int n_wave, char *lds,
+                                                   int wave, int lane) {
+  constexpr int WTN = NI * 32, VEC = 8;
+  constexpr int PITCH = WTN * 4 + 16, WBUF = 32 * PITCH;
+  constexpr int LPR = WTN / VEC, RPI = 64 / LPR; // lanes per row, rows per pass
+  static_assert(NWAVES * WBUF <= LDS_BYTES, "staging buffers must fit in the operand stages");
+  const RockEpilogue &e = p.epi;
+  const int lrow = lane & 31, lgrp = lane >> 5;
+  char *wbuf = lds + wave * WBUF;
+  const int rd_row = lane / LPR, rd_col = (lane % LPR) * VEC, n = n_wave + rd_col;
+  float s[VEC], b[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) { // (columns behind the last one: any value, they are not stored)
+    const int at = min(n + k, p.N - 1);
+    s[k] = p.channel_scale ? p.channel_scale[at] : e.scale;
+    b[k] = e.has_bias ? ((const float *)aux)[at] : 0.0f;
+  }
+  const float zero_point = (float)e.zero_point;
+  const bool vec_rows = out_rows_chunk_aligned(p, Cptr, out_elem_size(e.out_dtype)) && n + VEC <= p.N;
+  __builtin_amdgcn_s_barrier(); // every wave is done reading the operand stages
+  dispatch_tile_dtype<true>(p, [&](auto od_const) __attribute__((always_inline)) {
+    constexpr int OD = decltype(od_const)::value, ES = OutElemSize<OD>::value;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *(v4i *)(wbuf + lrow * PITCH + (j * 32 + q * 8 + lgrp * 4) * 4) =
+              v4i{acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+      RK_WAVE_LDS_ORDER();
+#pragma unroll
+      for (int r0 = 0; r0 < 32; r0 += RPI) {
+        const int row = r0 + rd_row, m = m_wave + i * 32 + row;
+        const v4i lo = *(const v4i *)(wbuf + row * PITCH + rd_col * 4);
+        const v4i hi = *(const v4i *)(wbuf + row * PITCH + rd_col * 4 + 16);
+        const float t = row_values(p, m).scale;
+        v4i out[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int sum = h ? hi[k] : lo[k];
+            v[k] = ((float)sum - zero_point) * s[4 * h + k] * t;
+            if (e.has_bias)
+              v[k] = v[k] + b[4 * h + k];
+            if (e.activation)
+              v[k] = activation_fast(v[k], e);
+          }
+          out[h] = epilogue_pack4<OD>(v, e);
+        }
+        if (m >= p.M)
+          continue;
+        char *dst = (char *)Cptr + ((int64_t)g * p.c_gs + (int64_t)m * p.c_ms + n) * ES;
+        if (vec_rows) {
+          if constexpr (ES == 4) {
+            *(v4i *)dst = out[0];
+            *(v4i *)(dst + 16) = out[1];
+          } else {
+            __builtin_nontemporal_store(v4i{out[0][0], out[0][1], out[1][0], out[1][1]}, (v4i *)dst);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            if (n + k < p.N) {
+              if constexpr (ES == 4)
+                ((int *)dst)[k] = out[k >> 2][k & 3];
+              else
+                ((uint16_t *)dst)[k] = (uint16_t)((uint32_t)out[k >> 2][(k >> 1) & 1] >> (16 * (k & 1)));
+            }
+        }
+      }
+      RK_WAVE_LDS_ORDER();
+    }
+  });
+}
+
+// ---- which tile a block works on ---------------------------------------------------------
+struct GroupTile {
+  int e, row0, rows, tm, tn; // group, its first row and row count, tile inside the group
+};
+
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane * 4, v); }
+
+// Boundaries that step back or lie outside [0, M] are read as if they stood at the furthest boundary before them, so
+// that whatever the offsets hold the groups are disjoint ranges of the M rows and every row tile is counted once.
+struct GroupScan {
+  int end, tiles; // running over the groups seen so far
+};
+// Lanes 0..63 take groups base..base+63: first row and row tiles before, up to and including the lane's group.
+template <int BM>
+__device__ __forceinline__ void scan_groups(const int32_t *offsets, int G, int M, int base, int lane, GroupScan &carry,
+                                            int &start, int &end, int &tiles_end) {
+  const int e = base + lane;
+  end = e < G ? min(max(offsets[e + 1], 0), M) : 0;
+  end = max(end, carry.end);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int before = lane_value(end, lane >= d ? lane - d : lane);
+    end = max(end, before);
+  }
+  start = lane_value(end, lane > 0 ? lane - 1 : 0);
+  start = lane > 0 ? start : carry.end;
+  tiles_end = (end - start + BM - 1) / BM;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int before = lane_value(tiles_end, lane >= d ? lane - d : lane);
+    tiles_end += lane >= d ? before : 0;
+  }
+  tiles_end += carry.tiles;
+  carry.end = __builtin_amdgcn_readfirstlane(lane_value(end, 63));
+  carry.tiles = __builtin_amdgcn_readfirstlane(lane_value(tiles_end, 63));
+}
+
+// The tile of this block; false: the block has none.  Uniform over the block: every wave computes the same.
+template <int BM>
+__device__ __forceinline__ bool locate_tile(const int32_t *offsets, const RockGemmParams &p, GroupTile &t) {
+  if (!offsets) {
+    int g;
+    decode_block(p.tiles_m, p.tiles_n, 1, p.group_m, p.xcd_remap, g, t.tm, t.tn);
+    t.e = 0;
+    t.row0 = 0;
+    t.rows = p.M;
+    return true;
+  }
+  const int lane = threadIdx.x & 63;
+  const GroupScan first = {__builtin_amdgcn_readfirstlane(min(max(offsets[0], 0), p.M)), 0};
+  GroupScan all = first;
+  int start, end, tiles_end;
+  for (int base = 0; base < p.G; base += 64)
+    scan_groups<BM>(offsets, p.G, p.M, base, lane, all, start, end, tiles_end);
+  // consecutive tiles on one XCD, as decode_block does it, over the tiles there are
+  const int total = all.tiles * p.tiles_n; // at most the grid: the groups are disjoint
+  int id = blockIdx.x;
+  if (id >= total)
+    return false;
+  const int per = total >> 3;
+  if (id < (per << 3))
+    id = (id & 7) * per + (id >> 3);
+  const int tile_row = id / p.tiles_n; // the group is found by it: a group's tiles are whole rows of tiles
+  int base = 0;
+  if (p.G > 64) {
+    GroupScan seen = first;
+    for (;; base += 64) { // (ends: tile_row < all.tiles, which the last pass reaches)
+      scan_groups<BM>(offsets, p.G, p.M, base, lane, seen, start, end, tiles_end);
+      if (tile_row < seen.tiles || base + 64 >= p.G)
+        break;
+    }
+  }
+  const uint64_t beyond = __builtin_amdgcn_ballot_w64(tiles_end > tile_row);
+  const int at = beyond ? __builtin_ctzll(beyond) : 63;
+  t.e = base + at;
+  t.row0 = __builtin_amdgcn_readfirstlane(lane_value(start, at));
+  t.rows = __builtin_amdgcn_readfirstlane(lane_value(end, at)) - t.row0;
+  const int tiles_m = (t.rows + BM - 1) / BM;
+  const int group_first = __builtin_amdgcn_readfirstlane(lane_value(tiles_end, at)) - tiles_m; // tile rows before the group
+  const int in_group = id - group_first * p.tiles_n;
+  // inside the group: blocks of group_m tile rows, walked down the columns, so that neighbours share operand tiles
+  const int group_sz = p.group_m * p.tiles_n;
+  const int grp = in_group / group_sz;
+  const int first_m = grp * p.group_m;
+  const int rows_here = min(tiles_m - first_m, p.group_m);
+  const int in_grp = in_group - grp * group_sz;
+  t.tm = first_m + in_grp % rows_here;
+  t.tn = in_grp / rows_here;
+  return true;
+}
+
+__device__ __forceinline__ int token_out_size(int od) { return od == ROCK_F32 ? 4 : 2; }
+
+// Moves the operands to the tile's group and calls f(A, B, C, bias, params).
+template <int DT, typename F>
+__device__ __forceinline__ void with_group(const void *A, const void *B, void *C, const void *bias,
+                                           const float *token_scale, const float *channel_scale,
+                                           const RockTokenGemmParams &tp, const GroupTile &t, F &&f) {
+  constexpr int ES = MmaTraits<DT>::ES;
+  const RockGemmParams &p = tp.gemm;
+  const void *a = (const char *)A + (int64_t)t.row0 * p.a_ms * ES;
+  const void *b = (const char *)B + (int64_t)t.e * p.b_gs * ES;
+  void *c = (char *)C + (int64_t)t.row0 * p.c_ms * token_out_size(p.epi.out_dtype);
+  if constexpr (MmaTraits<DT>::INT_ACC) {
+    TokenScaleParams q;
+    static_cast<RockGemmParams &>(q) = p;
+    q.M = t.rows;
+    q.token_scale = token_scale ? token_scale + t.row0 : nullptr;
+    q.channel_scale = channel_scale ? channel_scale + (int64_t)t.e * p.N : nullptr;
+    f(a, b, c, bias, q);
+  } else {
+    TokenTileParams q;
+    static_cast<RockGemmParams &>(q) = p;
+    q.M = t.rows;
+    f(a, b, c, bias, q);
+  }
+}
+
+template <int DT, int BM, int BN, int WM, int WN, int LB>
+__device__ __forceinline__ void token_gemm_body_dl(const void *A, const void *B, void *C, const void *bias,
+                                                   const int32_t *offsets, const float *token_scale,
+                                                   const float *channel_scale, const RockTokenGemmParams &tp) {
+  GroupTile t;
+  if (!locate_tile<BM>(offsets, tp.gemm, t))
+    return;
+  with_group<DT>(A, B, C, bias, token_scale, channel_scale, tp, t,
+                 [&](const void *a, const void *b, void *c, const void *x, const auto &q) __attribute__((always_inline)) {
+                   contraction_tile_dl<DT, BM, BN, WM, WN, 128, LD_ROWS_FAST, LB>(a, b, c, x, nullptr, q, 0, t.tm * BM,
+                                                                                  t.tn * BN);
+                 });
+}
+
+template <int DT, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void token_gemm_body_generic(const void *A, const void *B, void *C, const void *bias,
+                                                        const int32_t *offsets, const float *token_scale,
+                                                        const float *channel_scale, const RockTokenGemmParams &tp) {
+  GroupTile t;
+  if (!locate_tile<BM>(offsets, tp.gemm, t))
+    return;
+  with_group<DT>(A, B, C, bias, token_scale, channel_scale, tp, t,
+                 [&](const void *a, const void *b, void *c, const void *x, const auto &q) __attribute__((always_inline)) {
+                   contraction_tile<DT, BM, BN, WM, WN, LD_ROWS_GENERIC, LD_ROWS_GENERIC>(a, b, c, x, nullptr, q, 0,
+                                                                                          t.tm * BM, t.tn * BN);
+                 });
+}
+
+// ---- weight gradient -----------------------------------------------------------------------
+// (its own type: the loaders below instead of those for operands within one 2 GiB window)
+struct TokenWeightTile : TokenTileParams {};
+
+// ColsDl for a reduction over any number of rows: the buffer descriptor's base moves on with the K-steps in 64 bits
+// (scalar additions) and the lanes' offsets stay inside one stage.
+template <int DT, int COLS, int NW, int RB> struct ColsLongDl {
+  using Kg = KmGeom<DT, COLS, RB>;
+  struct Sg {
+    static constexpr int SLABS = COLS * RB / 1024;
+    static constexpr int PER_WAVE = SLABS / NW;
+    static_assert(SLABS % NW == 0, "stage must split into 1 KiB slabs per wave");
+  };
+  static constexpr int ES = Kg::ES;
+  const char *base;
+  int64_t step_bytes;         // between K-steps
+  unsigned off[Sg::PER_WAVE]; // byte offset of this lane's chunk inside a K-step, or kOobOffset
+  int krow[Sg::PER_WAVE];     // k-row of the chunk inside a stage
+  int K;
+  int wave;
+
+  __device__ __forceinline__ void init(const void *b, int64_t k_stride, int col0, int cols_total, int K_, int wave_,
+                                       int lane) {
+    wave = wave_;
+    K = K_;
+    base = (const char *)b + (int64_t)col0 * ES;
+    step_bytes = k_stride * ES * Kg::KR;
+#pragma unroll
+    for (int i = 0; i < Sg::PER_WAVE; ++i) {
+      const int idx = (wave * Sg::PER_WAVE + i) * 64 + lane; // physical chunk inside the stage
+      const int r = idx / Kg::CPR, pc = idx % Kg::CPR;
+      const int lc = pc ^ Kg::swz(r); // logical chunk this lane fetches
+      krow[i] = r;
+      const bool col_ok = col0 + (lc + 1) * (kChunk / ES) <= cols_total;
+      off[i] = col_ok ? (unsigned)(r * (int)k_stride * ES + lc * kChunk) : kOobOffset;
+    }
+  }
+  __device__ __forceinline__ void issue(int kt, char *stage) {
+    const __amdgpu_buffer_rsrc_t rsrc = dl_rsrc(base + kt * step_bytes);
+    const int k0 = kt * Kg::KR;
+#pragma unroll
+    for (int i = 0; i < Sg::PER_WAVE; ++i) {
+      const unsigned voff = (k0 + krow[i] < K) ? off[i] : kOobOffset;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          rsrc, (lds_void_t *)(stage + (wave * Sg::PER_WAVE + i) * 1024), 16, (int)voff, 0, 0, 0);
+    }
+  }
+};
+template <int DT, int ROWS, int NW, int RB, int KIND>
+__device__ __forceinline__ auto make_dl_a(const void *A, const TokenWeightTile &p, int, int m0, int wave, int lane) {
+  ColsLongDl<DT, ROWS, NW, RB> l;
+  l.init(A, p.a_ks, m0, p.M, p.K, wave, lane);
+  return l;
+}
+template <int DT, int ROWS, int NW, int RB, int KIND>
+__device__ __forceinline__ auto make_dl_b(const void *B, const TokenWeightTile &p, int, int n0, int wave, int lane) {
+  ColsLongDl<DT, ROWS, NW, RB> l;
+  l.init(B, p.b_ks, n0, p.N, p.K, wave, lane);
+  return l;
+}
+
+// Group g's rows as the reduction: operands and result moved to the group, gemm.K its number of rows
+template <int DT, typename F>
+__device__ __forceinline__ void with_weight_group(const void *A, const void *B, void *C, const int32_t *offsets,
+                                                  const RockTokenWeightParams &wp, int g, F &&f) {
+  constexpr int ES = MmaTraits<DT>::ES;
+  TokenWeightTile q;
+  static_cast<RockGemmParams &>(q) = wp.gemm;
+  const int lo = min(max(offsets[g], 0), q.K), hi = min(max(offsets[g + 1], lo), q.K);
+  q.K = __builtin_amdgcn_readfirstlane(hi - lo);
+  const int64_t row0 = __builtin_amdgcn_readfirstlane(lo);
+  f((const char *)A + row0 * q.a_ks * ES, (const char *)B + row0 * q.b_ks * ES,
+    (char *)C + (int64_t)g * q.c_gs * token_out_size(q.epi.out_dtype), q);
+}
+
+template <int DT, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void token_weight_body_dl(const void *A, const void *B, void *C, const int32_t *offsets,
+                                                     const RockTokenWeightParams &wp) {
+  int g, tm, tn;
+  decode_block(wp.gemm.tiles_m, wp.gemm.tiles_n, wp.gemm.G, wp.gemm.group_m, wp.gemm.xcd_remap, g, tm, tn);
+  with_weight_group<DT>(A, B, C, offsets, wp, g,
+                        [&](const void *a, const void *b, void *c, const TokenWeightTile &q)
+                            __attribute__((always_inline)) {
+                              contraction_tile_dl<DT, BM, BN, WM, WN, 128, LD_COLS_FAST, LD_COLS_FAST>(
+                                  a, b, c, nullptr, nullptr, q, 0, tm * BM, tn * BN);
+                            });
+}
+
+template <int DT, int BM, int BN, int WM, int WN>
+__device__ __forceinline__ void token_weight_body_generic(const void *A, const void *B, void *C,
+                                                          const int32_t *offsets, const RockTokenWeightParams &wp) {
+  int g, tm, tn;
+  decode_block(wp.gemm.tiles_m, wp.gemm.tiles_n, wp.gemm.G, wp.gemm.group_m, wp.gemm.xcd_remap, g, tm, tn);
+  with_weight_group<DT>(A, B, C, offsets, wp, g,
+                        [&](const void *a, const void *b, void *c, const TokenWeightTile &q)
+                            __attribute__((always_inline)) {
+                              contraction_tile<DT, BM, BN, WM, WN, LD_ROWS_GENERIC, LD_ROWS_GENERIC>(
+                                  a, b, c, nullptr, nullptr, static_cast<const TokenTileParams &>(q), 0, tm * BM,
+                                  tn * BN);
+                            });
+}
+
+} // namespace rk
+
+// ---- kernel-defining macros (rocmlir_amd/_build.py holds the list of kernels) -----------------
+#define RK_TG_CAT_(a, b) a##b
+#define RK_TG_CAT(a, b) RK_TG_CAT_(a, b)
+#define RK_TOKEN_GEMM_NAME(NAME) RK_TG_CAT(RK_TG_CAT(rock_token_gemm_, ROCK_DTNAME), NAME)
+#define RK_TOKEN_WEIGHT_NAME(NAME) RK_TG_CAT(RK_TG_CAT(rock_token_gemm_bwd_weight_, ROCK_DTNAME), NAME)
+#define RK_TOKEN_GEMM_ARGS                                                                            \
+  const void *A, const void *B, void *C, const void *bias, const int32_t *offsets,                    \
+      const float *token_scale, const float *channel_scale, RockTokenGemmParams p
+
+#define RK_TOKEN_GEMM_DL(NAME, BM, BN, WM, WN, LB)                                                    \
+  extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) { \
+    rk::token_gemm_body_dl<ROCK_DT, BM, BN, WM, WN, LB>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
+  }
+#define RK_TOKEN_GEMM(NAME, BM, BN, WM, WN)                                                           \
+  extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) { \
+    rk::token_gemm_body_generic<ROCK_DT, BM, BN, WM, WN>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
+  }
+#define RK_TOKEN_WEIGHT_DL(NAME, BM, BN, WM, WN)                                                      \
+  extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_WEIGHT_NAME(NAME)(               \
+      const void *A, const void *B, void *C, const int32_t *offsets, RockTokenWeightParams p) {       \
+    rk::token_weight_body_dl<ROCK_DT, BM, BN, WM, WN>(A, B, C, offsets, p);                           \
+  }
+#define RK_TOKEN_WEIGHT(NAME, BM, BN, WM, WN)                                                         \
+  extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_WEIGHT_NAME(NAME)(               \
+      const void *A, const void *B, void *C, const int32_t *offsets, RockTokenWeightParams p) {       \
+    rk::token_weight_body_generic<ROCK_DT, BM, BN, WM, WN>(A, B, C, offsets, p);                      \
+  }

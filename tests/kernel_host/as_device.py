@@ -33,7 +33,7 @@ def _the_model():
         so = os.path.join(d, "libkernel_host.so")
         if not os.path.exists(so):
             os.makedirs(d, exist_ok=True)
-            km.build_model(d, types=km.ALL_TYPES, rolled=True)
+            km.build_model(d, types=km.ALL_TYPES, rolled=True, tokens=tuple(km._build.TOKEN_TYPES))
         _model = km.load_model(so)
         _model.hm_set_late_loads(int(os.environ.get("ROCK_HOST_LATE_LOADS", "0")))
         _model.hm_set_thread_order(int(os.environ.get("ROCK_HOST_THREAD_ORDER", "0")))

@@ -91,6 +91,43 @@ def _attention_sources(parts=4):
     return units
 
 
+def _token_sources(code):
+    """The products of token rows of one operand type (csrc/token_gemm.h): rows, weights, result, bias, offsets, token
+    scales, channel scales; weight gradient: operands, result, offsets."""
+    t = _build.TOKEN_TYPES[code]
+    kernels = _build.token_kernels(code)
+    units = {}
+    for part in range(3):
+        mine = kernels[part::3]
+        lines = ["#define ROCK_DT %d" % code, "#define ROCK_DTNAME %s" % t, '#include "token_gemm.h"',
+                 '#include "kernel_table.h"', "#include <cstring>"]
+        lines += [m for _, m in mine]
+        for n, m in mine:
+            if "WEIGHT" in m:
+                ptype, args = "RockTokenWeightParams", "q[0], q[1], q[2], (const int32_t *)q[3]"
+            else:
+                ptype = "RockTokenGemmParams"
+                args = "q[0], q[1], q[2], q[3], (const int32_t *)q[4], (const float *)q[5], (const float *)q[6]"
+            lines.append("static void call_%s(void **q, const void *params) { %s p; std::memcpy(&p, params, sizeof p); "
+                         "%s(%s, p); }" % (n, ptype, n, args))
+        lines.append("static const HmEntry table[] = {")
+        lines += ['  {"%s", call_%s},' % (n, n) for n, _ in mine]
+        lines += ["  {nullptr, nullptr}};", "const HmEntry *hm_table_token_%s_%d() { return table; }" % (t, part)]
+        units["model_token_%s_%d" % (t, part)] = "\n".join(lines) + "\n"
+    return units
+
+
+def _quantize_source():
+    lines = ['#include "quantize_tokens.hip"', '#include "kernel_table.h"', "#include <cstring>"]
+    for n in _build.QUANTIZE_KERNELS:
+        lines.append("static void call_%s(void **q, const void *params) { RockQuantizeParams p; std::memcpy(&p, params, "
+                     "sizeof p); %s(q[0], q[1], q[2], p); }" % (n, n))
+    lines.append("static const HmEntry table[] = {")
+    lines += ['  {"%s", call_%s},' % (n, n) for n in _build.QUANTIZE_KERNELS]
+    lines += ["  {nullptr, nullptr}};", "const HmEntry *hm_table_quantize() { return table; }"]
+    return "\n".join(lines) + "\n"
+
+
 def _table_source(tables):
     lines = ['#include "kernel_table.h"', "#include <vector>"]
     lines += ["const HmEntry *%s();" % t for t in tables]
@@ -100,16 +137,21 @@ def _table_source(tables):
     return "\n".join(lines) + "\n"
 
 
-def build_model(d, types=(0, 1), rolled=False, attention=True):
+def build_model(d, types=(0, 1), rolled=False, attention=True, tokens=()):
     """Compiles the model into directory d and returns the loaded library.  types: operand type codes (f32 and
     f16 by default; ALL_TYPES for every one); rolled: the kernels with the rolled epilogue ("_e": same loads and
-    tiles, their own store code) too; attention: the fused attention kernels."""
+    tiles, their own store code) too; attention: the fused attention kernels; tokens: operand type codes of the products
+    of token rows (and, with any, the quantisation kernels)."""
     assert CLANG, "the host build uses clang's vector extensions"
     units = {"model_utility": _utility_source()}
     for code in types:
         units.update(_model_sources(code, rolled))
     if attention:
         units.update(_attention_sources())
+    for code in tokens:
+        units.update(_token_sources(code))
+    if tokens:
+        units["model_quantize"] = _quantize_source()
     units["kernel_table"] = _table_source(["hm_table_" + n[len("model_"):] for n in units])
     for name, text in units.items():
         with open(os.path.join(d, name + ".cpp"), "w") as f:

@@ -1,0 +1,247 @@
+"""The kernels over token rows (csrc/token_gemm.h, csrc/quantize_tokens.hip) built for the CPU and run through whole
+plans: every address checked, loads landing at issue or at their wait, no byte written by two blocks, and on
+integer-valued data results equal to numpy's bit for bit.  The plans come from the C ABI as a caller gets them."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+from tests.kernel_host.model import CLANG, build_model, run_plan  # noqa: E402
+
+pytestmark = pytest.mark.skipif(CLANG is None, reason="the host build uses clang's vector extensions")
+
+_NUMPY = {"f32": np.float32, "f16": np.float16, "i8": np.int8}
+
+
+@pytest.fixture(scope="module")
+def model(tmp_path_factory):
+    lib = build_model(str(tmp_path_factory.mktemp("kernel_host_tokens")), types=(), attention=False, tokens=(0, 1, 3))
+    lib.hm_set_owner_check(1)
+    return lib
+
+
+@pytest.fixture(params=["loads-land-at-issue", "loads-land-at-the-wait"])
+def loads(request, model):
+    late = request.param == "loads-land-at-the-wait"
+    model.hm_set_late_loads(1 if late else 0)
+    model.hm_set_thread_order(2 if late else 0)
+    yield request.param
+    model.hm_set_late_loads(0)
+    model.hm_set_thread_order(0)
+
+
+@pytest.fixture(scope="module")
+def rock():
+    import rocmlir_amd
+    rocmlir_amd.load_library()
+    return rocmlir_amd
+
+
+def bounds(offsets, T):
+    """The groups' rows as the operators read them: offsets clamped to the rows, none before one in front of it."""
+    at = np.maximum.accumulate(np.clip(np.asarray(offsets, np.int64), 0, T))
+    return list(zip(at[:-1], at[1:]))
+
+
+def flag(b):
+    return str(bool(b)).lower()
+
+
+# ---- quantisation ---------------------------------------------------------------------------------------------
+def quantise_reference(x):
+    """The definition in 64 bits: roundeven(127 x / max), and max / 127 rounded to f32 once."""
+    x = x.astype(np.float64)
+    top = np.abs(x).max(axis=1)
+    bad = ~np.isfinite(x).all(axis=1)
+    unit = np.where(bad | (top == 0), 1.0, top)
+    q = np.where(bad[:, None], 0.0, np.rint(127.0 * np.where(bad[:, None], 0.0, x) / unit[:, None])).astype(np.int8)
+    scale = (top.astype(np.float32) / np.float32(127.0)).astype(np.float32)
+    scale[bad] = np.nan
+    return q, scale
+
+
+@pytest.mark.parametrize("t", ["f32", "f16"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 64), (9, 513), (1030, 24), (2, 4100), (1027, 4104), (1, 20000)])
+def test_quantisation_equals_the_definition(model, rock, t, rows, cols):
+    rng = np.random.default_rng(rows * 31 + cols)
+    x = (rng.standard_normal((rows, cols)) * np.exp(rng.uniform(-3, 3, (rows, 1)))).astype(_NUMPY[t])
+    # ties: whole and half steps of a row whose largest magnitude is 127 (or 254, where odd values are halves)
+    x[0] = (rng.integers(-254, 255, cols)).astype(_NUMPY[t])
+    x[0, 0] = 254
+    if rows > 2:
+        x[1] = 0
+        x[2, cols // 2] = np.inf
+    if rows > 4:
+        x[3, cols - 1] = np.nan
+        x[4] = x[4] * _NUMPY[t](1e-6)      # f16: subnormal
+    if rows > 8 and t == "f32":
+        x[5] = (x[5].astype(np.float64) * 1e-38).astype(np.float32)   # 127 / max overflows
+        x[6] = (x[6].astype(np.float64) * 1e36).astype(np.float32)
+    names, problems, out = run_plan(model, rock, "-operation quantize_tokens -t %s -m %d -k %d" % (t, rows, cols), {0: x})
+    assert names == ["rock_quantize_tokens_" + t] and not problems, (names, problems)
+    q, scale = quantise_reference(x)
+    assert np.array_equal(out[1][:q.size].view(np.int8).reshape(q.shape), q)
+    assert np.array_equal(out[2][:4 * rows].view(np.float32), scale, equal_nan=True)
+
+
+# ---- int8 product with token and channel scales -----------------------------------------------------------------
+def scaled(acc, zp, channel, token, bias, out):
+    """The epilogue, one f32 operation per step."""
+    v = (acc.astype(np.float32) - np.float32(zp)) * channel.astype(np.float32)
+    v = (v * token[:, None].astype(np.float32)).astype(np.float32)
+    if bias is not None:
+        v = v + bias[None, :].astype(np.float32)
+    return v.astype(_NUMPY[out])
+
+
+@pytest.mark.parametrize("shape,transB,extra", [
+    ((1, 64, 128), True, ""), ((70, 45, 96), True, ""), ((33, 40, 100), True, ""), ((50, 48, 64), False, ""),
+    ((20, 33, 48), False, ""), ((300, 260, 144), True, "-perf_config v2:256,256"), ((130, 200, 272), True, "-perf_config v2:128,128"),
+    ((130, 208, 80), False, "-perf_config v2:128,128"), ((260, 272, 160), False, "-perf_config v2:256,256")],
+    ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else None)
+@pytest.mark.parametrize("out,vector,bias", [("f16", True, True), ("f32", False, False)])
+def test_int8_product_with_token_scales(model, rock, loads, shape, transB, extra, out, vector, bias):
+    m, n, k = shape
+    rng = np.random.default_rng(m + n + k)
+    A = rng.integers(-128, 128, (m, k)).astype(np.int8)
+    B = rng.integers(-128, 128, (n, k) if transB else (k, n)).astype(np.int8)
+    token = rng.uniform(0.001, 0.01, m).astype(np.float32)
+    channel = rng.uniform(0.01, 0.1, n).astype(np.float32)
+    bv = rng.integers(-4, 5, n).astype(np.float32)
+    opts = ("-operation gemm -arch gfx950 -t i8 -m %d -n %d -k %d -transB %s -out_datatype %s -token_scale_vector true -zero_point 3 %s"
+            % (m, n, k, flag(transB), out, extra))
+    inputs = {0: A, 1: B, 4: token}
+    if vector:
+        opts += " -scale_vector true"
+        inputs[5] = channel
+    else:
+        opts += " -scale 0.03125 -activation clip -clip_min -2 -clip_max 3"
+    if bias:
+        opts += " -bias true"
+        inputs[3] = bv
+    names, problems, got = run_plan(model, rock, opts, inputs)
+    assert not problems, (names, problems)
+    acc = A.astype(np.int64) @ (B.T if transB else B).astype(np.int64)
+    want = scaled(acc, 3, channel if vector else np.full(n, 0.03125), token, bv if bias else None, "f32")
+    if not vector:
+        want = np.clip(want, -2, 3)
+    want = want.astype(_NUMPY[out])
+    assert np.array_equal(got[2][:want.nbytes].view(want.dtype).reshape(m, n), want), names
+
+
+# ---- products grouped by expert -----------------------------------------------------------------------------------
+# (groups' sizes, rows behind the last group, N, K): empty groups, one row, tiles that end inside a group, 70 groups
+GROUPS = [([5], 0, 24, 32), ([0, 3, 0, 64, 1, 0], 3, 40, 64), ([130, 0, 7], 5, 72, 48), ([0, 0], 4, 16, 32),
+          ([1] * 70 + [0, 9], 2, 16, 32), ([17, 40], 0, 33, 35), ([3, 66, 2], 1, 77, 64)]
+
+
+def _problem(sizes, tail, n, k, t, transB, seed=0):
+    rng = np.random.default_rng(seed + sum(sizes))
+    T = sum(sizes) + tail
+    offsets = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    E = len(sizes)
+    x = rng.integers(-3, 4, (T, k)).astype(_NUMPY[t])
+    w = rng.integers(-3, 4, (E, n, k) if transB else (E, k, n)).astype(_NUMPY[t])
+    return rng, T, E, offsets, x, w
+
+
+def _opts(op, t, T, E, n, k, transB, extra=""):
+    return "-operation %s -arch gfx950 -t %s -g %d -m %d -n %d -k %d -transB %s %s" % (op, t, E, T, n, k, flag(transB), extra)
+
+
+@pytest.mark.parametrize("case", GROUPS, ids=lambda c: "%dgroups-%dx%d" % (len(c[0]), c[2], c[3]))
+@pytest.mark.parametrize("t,transB", [("f16", True), ("f16", False), ("f32", True), ("i8", True), ("i8", False)])
+def test_grouped_product(model, rock, loads, case, t, transB):
+    sizes, tail, n, k = case
+    rng, T, E, offsets, x, w = _problem(sizes, tail, n, k, t, transB)
+    inputs, extra, out = {0: x, 1: w, 3: offsets}, "", t
+    if t == "i8":
+        token, channel = rng.uniform(0.5, 1, T).astype(np.float32), rng.uniform(0.1, 0.5, (E, n)).astype(np.float32)
+        inputs.update({4: token, 5: channel})
+        extra, out = "-token_scale_vector true -scale_vector true -out_datatype f32", "f32"
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm", t, T, E, n, k, transB, extra), inputs)
+    assert not problems, (names, problems)
+    res = got[2][:T * n * np.dtype(_NUMPY[out]).itemsize].view(_NUMPY[out]).reshape(T, n)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        acc = x[a:b].astype(np.float64) @ (w[e].T if transB else w[e]).astype(np.float64)
+        want = scaled(acc, 0, channel[e], token[a:b], None, "f32") if t == "i8" else acc
+        assert np.array_equal(res[a:b].astype(np.float64), want.astype(np.float64)), (names, e)
+    assert (res[sum(sizes):].view(np.uint8) == 0xEE).all(), "rows behind the last group were written"
+
+
+@pytest.mark.parametrize("case", GROUPS, ids=lambda c: "%dgroups-%dx%d" % (len(c[0]), c[2], c[3]))
+@pytest.mark.parametrize("t,transB", [("f16", True), ("f16", False), ("f32", True)])
+def test_grouped_gradients(model, rock, loads, case, t, transB):
+    sizes, tail, n, k = case
+    rng, T, E, offsets, x, w = _problem(sizes, tail, n, k, t, transB)
+    dout = rng.integers(-3, 4, (T, n)).astype(_NUMPY[t])
+    dout[sum(sizes):] = np.nan      # rows of no group: read by nothing
+    x[sum(sizes):] = np.nan
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_data", t, T, E, n, k, transB),
+                                    {1: w, 2: dout, 3: offsets})
+    assert not problems, (names, problems)
+    dx = got[0][:x.nbytes].view(x.dtype).reshape(T, k).copy()   # (the next plan reuses the memory)
+    names_w, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_weight", t, T, E, n, k, transB),
+                                      {0: x, 2: dout, 3: offsets})
+    assert not problems, (names_w, problems)
+    dw = got[1][:w.nbytes].view(w.dtype).reshape(w.shape)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        we = (w[e] if transB else w[e].T).astype(np.float64)     # [N, K]
+        d64, x64 = dout[a:b].astype(np.float64), x[a:b].astype(np.float64)
+        assert np.array_equal(dx[a:b].astype(np.float64), d64 @ we), (names, e)
+        want = d64.T @ x64 if transB else x64.T @ d64
+        assert np.array_equal(dw[e].astype(np.float64), want), (names_w, e)
+    assert (dx[sum(sizes):].view(np.uint8) == 0xEE).all()
+
+
+@pytest.mark.parametrize("tile", ["v2:256,256", "v2:128,128", "v2:64,64"])
+@pytest.mark.parametrize("t,transB", [("f16", True), ("f16", False), ("i8", True)])
+def test_grouped_product_every_tile(model, rock, loads, tile, t, transB):
+    """Groups that end inside a tile, at a tile's end and one row behind it, on every tile."""
+    sizes, tail, n, k = [64, 0, 129, 257, 1], 2, 272, 80
+    rng, T, E, offsets, x, w = _problem(sizes, tail, n, k, t, transB)
+    extra = "-perf_config " + tile + (" -out_datatype f32" if t == "i8" else "")
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm", t, T, E, n, k, transB, extra),
+                                    {0: x, 1: w, 3: offsets})
+    assert not problems and tile[3:].replace(",", "x") in names[0], (names, problems)
+    out = np.float32 if t == "i8" else _NUMPY[t]
+    res = got[2][:T * n * np.dtype(out).itemsize].view(out).reshape(T, n)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        assert np.array_equal(res[a:b].astype(np.float64), x[a:b].astype(np.float64) @ (w[e].T if transB else w[e]).astype(np.float64)), e
+
+
+@pytest.mark.parametrize("tile", ["v2:256,256", "v2:128,128", "v2:64,64"])
+def test_grouped_weight_gradient_every_tile(model, rock, loads, tile):
+    sizes, tail, n, k = [64, 0, 129, 1], 2, 272, 136
+    rng, T, E, offsets, x, w = _problem(sizes, tail, n, k, "f16", True)
+    dout = rng.integers(-3, 4, (T, n)).astype(np.float16)
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_weight", "f16", T, E, n, k, True, "-perf_config " + tile),
+                                    {0: x, 2: dout, 3: offsets})
+    assert not problems and tile[3:].replace(",", "x") in names[0], (names, problems)
+    dw = got[1][:w.nbytes].view(w.dtype).reshape(w.shape)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        assert np.array_equal(dw[e].astype(np.float64), dout[a:b].astype(np.float64).T @ x[a:b].astype(np.float64)), e
+
+
+@pytest.mark.parametrize("offsets", [[0, 5, 3, 9], [-4, 2, 100, 7], [4, 4, 4, 2], [9, 0, 0, 0], [2147483647] * 4, [-2147483648, 1, 1, 12]])
+def test_offsets_that_are_no_offsets_stay_inside_the_tensors(model, rock, offsets):
+    """Boundaries that step back or lie outside are read as the furthest one before them: nothing outside the tensors
+    is touched, no row belongs to two groups."""
+    T, n, k = 12, 24, 32
+    rng = np.random.default_rng(5)
+    x, w = rng.integers(-3, 4, (T, k)).astype(np.float16), rng.integers(-3, 4, (3, n, k)).astype(np.float16)
+    dout = rng.integers(-3, 4, (T, n)).astype(np.float16)
+    off = np.asarray(offsets, np.int64).astype(np.int32)
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm", "f16", T, 3, n, k, True), {0: x, 1: w, 3: off})
+    assert not problems, (names, problems)
+    res = got[2][:T * n * 2].view(np.float16).reshape(T, n)
+    owned = np.zeros(T, bool)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        assert np.array_equal(res[a:b].astype(np.float64), x[a:b].astype(np.float64) @ w[e].T.astype(np.float64))
+        owned[a:b] = True
+    assert (res[~owned].view(np.uint8) == 0xEE).all()
+    for op, inputs in (("grouped_gemm_bwd_data", {1: w, 2: dout, 3: off}), ("grouped_gemm_bwd_weight", {0: x, 2: dout, 3: off})):
+        names, problems, _ = run_plan(model, rock, _opts(op, "f16", T, 3, n, k, True), inputs)
+        assert not problems, (names, problems)

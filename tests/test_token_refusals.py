@@ -1,0 +1,104 @@
+"""What the operators over token rows refuse, on the host, before anything is launched: through the package's entry points
+(with tensors on the CPU, which get no further than the checks) and through option strings."""
+import pytest
+import torch
+
+
+def _t(*shape, dtype=torch.float16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+OFF3 = torch.zeros(4, dtype=torch.int32)
+I8 = torch.int8
+
+
+@pytest.mark.parametrize("call,text", [
+    (lambda r: r.quantize_tokens(_t(4, 8, dtype=torch.int8)), "f16, bf16 or f32"),
+    (lambda r: r.quantize_tokens(torch.tensor(1.0)), "f16, bf16 or f32"),
+    (lambda r: r.quantize_tokens(_t(4, 8), out=_t(4, 8)), "out must be"),
+    (lambda r: r.quantize_tokens(_t(4, 8), out=_t(8, 4, dtype=I8).t()), "contiguous"),
+    (lambda r: r.quantize_tokens(_t(4, 8), scale_out=_t(4)), "out must be"),
+    (lambda r: r.gemm(_t(4, 8), _t(6, 8), transB=True, token_scale=torch.ones(4)), "int8 operands"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 8, dtype=I8), transB=True, token_scale=torch.ones(6)), "token_scale must hold 4"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 8, dtype=I8), transB=True, token_scale=torch.ones(4).half()), "token_scale must hold"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 8, dtype=I8), transB=True, token_scale=torch.ones(4), scale=torch.ones(4)), "scale must hold 6"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 8, dtype=I8), transB=True, token_scale=torch.ones(4), bias=torch.ones(4)), "bias must hold 6"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 9, dtype=I8), transB=True, token_scale=torch.ones(4)), "shapes do not match"),
+    (lambda r: r.gemm(_t(2, 4, 8, dtype=I8), _t(2, 6, 8, dtype=I8), transB=True, token_scale=torch.ones(4)), "one batch entry"),
+    (lambda r: r.gemm(_t(8, 4, dtype=I8), _t(6, 8, dtype=I8), transA=True, transB=True, token_scale=torch.ones(4)), "takes scale"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 8, dtype=I8), transB=True, token_scale=torch.ones(4), residual=_t(4, 6)), "takes scale"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 8, dtype=I8), transB=True, token_scale=torch.ones(4), out_dtype="i32"), "out_dtype"),
+    (lambda r: r.gemm(_t(4, 8, dtype=I8), _t(6, 8, dtype=I8), transB=True, token_scale=torch.ones(4), activation="gelu"), "relu and clip"),
+    (lambda r: r.gemm(_t(1, 131072, dtype=I8), _t(1, 131072, dtype=I8), transB=True, token_scale=torch.ones(1)), "131071"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3.long(), transB=True), "offsets is int32"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3[:3], transB=True), "offsets is int32"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(0, 6, 8), OFF3[:1], transB=True), "no experts"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3), "shapes do not match"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8, dtype=torch.bfloat16), OFF3, transB=True), "of one type"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3, transB=True, scale=2.0), "scales go with int8"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3, transB=True, token_scale=torch.ones(5)), "scales go with int8"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3, transB=True, out_dtype="i8"), "out_dtype"),
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3, transB=True, out=_t(5, 8)), "out must be"),
+    (lambda r: r.grouped_gemm(_t(5, 8, dtype=I8), _t(3, 6, 8, dtype=I8), OFF3, transB=True, scale=torch.ones(6)), "scale must hold 18"),
+    (lambda r: r.grouped_gemm(_t(5, 8, dtype=torch.float64), _t(3, 6, 8, dtype=torch.float64), OFF3, transB=True), "unsupported tensor dtype"),
+    (lambda r: r.grouped_gemm_bwd_data(_t(5, 8), _t(3, 6, 8), OFF3, transB=True), "shapes do not match"),
+    (lambda r: r.grouped_gemm_bwd_data(_t(5, 6, dtype=I8), _t(3, 6, 8, dtype=I8), OFF3, transB=True), "f16, bf16 or f32"),
+    (lambda r: r.grouped_gemm_bwd_weight(_t(5, 8), _t(4, 6), OFF3), "of one type"),
+    (lambda r: r.grouped_gemm_bwd_weight(_t(5, 8), _t(5, 6), OFF3, out=_t(3, 6, 8)), "out must be"),
+    (lambda r: r.grouped_gemm_bwd_weight(_t(5, 8), _t(5, 6), OFF3.float()), "offsets is int32"),
+    # tensors that pass every check but do not live on a GPU
+    (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3, transB=True), "must live on the GPU"),
+    (lambda r: r.quantize_tokens(_t(5, 8)), "must live on the GPU"),
+], ids=lambda v: v.replace(" ", "-") if isinstance(v, str) else "")
+def test_entry_points_refuse(rock, call, text):
+    with pytest.raises(rock.RockError, match=text):
+        call(rock)
+
+
+@pytest.mark.parametrize("options,text", [
+    ("-operation quantize_tokens -t i8 -m 4 -k 4", "quantize_tokens"),
+    ("-operation quantize_tokens -t f16 -m 0 -k 4", "positive"),
+    ("-operation quantize_tokens -t f16 -m 4", "positive"),
+    ("-operation quantize_tokens -t f16 -m 4 -k 4 -kernel_id 1", "kernel_id"),
+    ("-operation grouped_gemm -t fp8 -g 2 -m 4 -n 8 -k 16", "operands are"),
+    ("-operation grouped_gemm -t f16 -g 0 -m 4 -n 8 -k 16", "positive"),
+    ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8", "positive"),
+    ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8 -k 16 -transA true", "no transA"),
+    ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8 -k 16 -bias true", "no bias"),
+    ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8 -k 16 -token_scale_vector true", "scales go with int8"),
+    ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8 -k 16 -out_datatype i8", "the result is"),
+    ("-operation grouped_gemm -t f16 -g 2 -m 2147483000 -n 2147483000 -k 16", "more tiles"),
+    ("-operation grouped_gemm_bwd_weight -t i8 -g 2 -m 4 -n 8 -k 16", "gradients take"),
+    ("-operation grouped_gemm_bwd_data -t f16 -g 2 -m 4 -n 8 -k 16 -out_datatype f32", "its tensor's type"),
+    ("-operation gemm -t i8 -g 2 -m 4 -n 8 -k 16 -token_scale_vector true", "one batch entry"),
+    ("-operation gemm -t f16 -m 4 -n 8 -k 16 -token_scale_vector true", "int8 operands"),
+    ("-operation gemm -t i8 -m 4 -n 8 -k 16 -token_scale_vector true -activation tanh", "relu and clip"),
+    ("-operation gemm -t i8 -m 4 -n 8 -k 16 -token_scale_vector true -residual add", "no residual"),
+    ("-operation gemm -t i8 -m 4 -n 8 -k 16 -token_scale_vector true -store-method atomic_add", "token scales"),
+    ("-operation conv -t i8 -token_scale_vector true", "gemm and grouped_gemm only"),
+])
+def test_option_strings_refuse(rock, options, text):
+    with pytest.raises(rock.RockError, match=text):
+        rock.RockKernel(options)
+
+
+def test_argument_sizes_are_checked(rock):
+    """rockamdCheckArgumentSizes knows every tensor of the new operators."""
+    import ctypes as C
+    k = rock.RockKernel("-operation grouped_gemm -t i8 -g 3 -m 5 -n 8 -k 16 -transB true -token_scale_vector true -scale_vector true")
+    need = [5 * 16, 3 * 8 * 16, 5 * 8 * 2, 4 * 4, 5 * 4, 3 * 8 * 4]
+    lib = rock.load_library()
+    assert lib.rockamdCheckArgumentSizes(k._h, (C.c_size_t * 6)(*need), 6) == 0
+    for i in range(6):
+        short = list(need)
+        short[i] -= 1
+        assert lib.rockamdCheckArgumentSizes(k._h, (C.c_size_t * 6)(*short), 6) != 0, i
+
+
+def test_tuning_space_of_the_new_operators(rock):
+    k = rock.RockKernel("-operation grouped_gemm -t f16 -g 3 -m 500 -n 256 -k 64 -transB true")
+    space = k.tuning_space()
+    assert len(space) >= 3
+    for perf in space:
+        assert rock.RockKernel(k.options + " -perf_config " + perf).perf_config == perf
+    assert len(rock.RockKernel("-operation quantize_tokens -t f16 -m 5 -k 8").tuning_space()) == 1
