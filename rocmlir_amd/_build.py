@@ -109,6 +109,8 @@ def attention_kernels():
     return out
 
 
+# kernels for few token rows: 16-row tiles, 16-column tiles, K-steps of loads in flight
+TOKEN_SKINNY = ((1, 1, 8), (1, 2, 8), (2, 1, 8), (2, 2, 4), (4, 2, 4))
 TOKEN_TYPES = {0: "f32", 1: "f16", 2: "bf16", 3: "i8"}
 
 
@@ -122,9 +124,14 @@ def token_kernels(type_code):
         out.append(("rock_token_gemm_%s%s_fast_nn" % (t, tile), "RK_TOKEN_GEMM_DL(%s_fast_nn, %s, %s)" % (tile, dims, COLS)))
         if t != "i8":
             out.append(("rock_token_gemm_bwd_weight_%s%s" % (t, tile), "RK_TOKEN_WEIGHT_DL(%s, %s)" % (tile, dims)))
-    out.append(("rock_token_gemm_%s_64x64_generic" % t, "RK_TOKEN_GEMM(_64x64_generic, 64, 64, 2, 2)"))
+    for b_cols in (False, True):     # rows of any alignment
+        name = "_64x64_any" + ("_nn" if b_cols else "")
+        out.append(("rock_token_gemm_%s%s" % (t, name), "RK_TOKEN_GEMM_ANY(%s, 64, 64, 2, 2, %s)" % (name, str(b_cols).lower())))
+    for mt, ct, unroll in TOKEN_SKINNY:
+        name = "_%dx%d_skinny" % (16 * mt, 16 * ct)
+        out.append(("rock_token_gemm_%s%s" % (t, name), "RK_TOKEN_GEMM_SKINNY(%s, %d, %d, %d)" % (name, mt, ct, unroll)))
     if t != "i8":
-        out.append(("rock_token_gemm_bwd_weight_%s_64x64_generic" % t, "RK_TOKEN_WEIGHT(_64x64_generic, 64, 64, 2, 2)"))
+        out.append(("rock_token_gemm_bwd_weight_%s_64x64_any" % t, "RK_TOKEN_WEIGHT_ANY(_64x64_any, 64, 64, 2, 2)"))
     return out
 
 

@@ -323,6 +323,20 @@ class RockKernel:
             raise RockError("launch of %s failed (hip error %d): %s"
                             % (self.kernel_name, rc, last_error()))
 
+    def launch_checked(self, args):
+        """launch() on torch's current stream for a caller that has checked the tensors against the problem's sizes
+        and made their device the current one: a call costs the host a third of launch()."""
+        import torch
+        arr = (C.c_void_p * len(args))()
+        for i, a in enumerate(args):
+            if a is not None:
+                if not a.is_cuda:
+                    raise RockError("tensor arguments must live on the GPU")
+                arr[i] = a.data_ptr()
+        rc = _lib.rockamdLaunch(self._h, arr, len(args), torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+        if rc != 0:
+            raise RockError("launch of %s failed (hip error %d): %s" % (self.kernel_name, rc, last_error()))
+
     def benchmark(self, *args, warmup=3, iters=20, stream=None):
         """Average milliseconds per launch (HIP events on the launch stream)."""
         arr = self._pointer_array(args)
@@ -900,12 +914,16 @@ def conv2d_bwd_weight(inp, dout, *, fil_layout, in_layout, out_layout, batchsize
 _token_plans = {}
 
 
-def _token_plan(*key):
-    """The plan of a problem given as (operation, type, (option, value), ...); `key` is its cache entry."""
+def _token_plan(operation, t, **options):
+    """The plan of a problem (options that are None or False are left out)."""
+    key = (operation, t) + tuple(options.items())
     p = _token_plans.get(key)
     if p is None:
-        opts = "-operation %s -arch gfx950 -t %s" % key[:2] + "".join(" -%s %s" % kv for kv in key[2:] if kv[1] is not None)
-        p = RockProgram(opts)
+        text = "-operation %s -arch gfx950 -t %s" % (operation, t)
+        for k, v in options.items():
+            if v is not None and v is not False:
+                text += " -%s %s" % (k, "true" if v is True else "%.9g" % v if isinstance(v, float) else v)
+        p = RockProgram(text)
         if len(_token_plans) >= 4096:   # token counts change from call to call
             _token_plans.clear()
         _token_plans[key] = p
@@ -914,63 +932,66 @@ def _token_plan(*key):
 
 def _dense(t):
     """`t` as the kernels address it: contiguous, from a 16-byte boundary on."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
 
 
-class _TokenCall:
-    """Where the tensors' work runs: their device is made the current one, `stream` (default: the device's current
-    stream) torch's current stream, so that copies and results made on the way are ordered with the kernels."""
+def _same_device(name, first, **others):
+    for what, t in others.items():
+        if t is not None and t.device != first.device:
+            raise RockError("%s: %s is on %s, the first operand on %s" % (name, what, t.device, first.device))
 
-    def __init__(self, name, stream, **tensors):
-        self.name = name
-        self.device = next(t.device for t in tensors.values() if t is not None)
-        for what, t in tensors.items():
-            if t is not None and t.device != self.device:
-                raise RockError("%s: %s is on %s, the other tensors on %s" % (name, what, t.device, self.device))
+
+class _on:
+    """Makes the operands' device the current one and `stream` (default: the device's current stream) torch's current
+    stream, so that copies and results made on the way are ordered with the kernels."""
+
+    def __init__(self, name, device, stream):
         self._contexts = []
-        if self.device.type == "cuda":
-            import torch
-            if self.device.index != torch.cuda.current_device():
-                self._contexts.append(torch.cuda.device(self.device))
-            if stream is not None:
-                if not isinstance(stream, torch.cuda.Stream):
-                    stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=self.device)
-                if stream.device != self.device:
-                    raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, self.device))
-                self._contexts.append(torch.cuda.stream(stream))
+        if device.type != "cuda":
+            return
+        import torch
+        if device.index != torch.cuda.current_device():
+            self._contexts.append(torch.cuda.device(device))
+        if stream is not None:
+            if not isinstance(stream, torch.cuda.Stream):
+                stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=device)
+            if stream.device != device:
+                raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, device))
+            self._contexts.append(torch.cuda.stream(stream))
 
     def __enter__(self):
         for c in self._contexts:
             c.__enter__()
-        return self
 
     def __exit__(self, *exc):
         for c in reversed(self._contexts):
             c.__exit__(*exc)
 
-    def result(self, out, shape, dtype):
-        """`out` checked, or a new tensor."""
-        import torch
-        if out is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
-        if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != self.device:
-            raise RockError("%s: out must be %s of %s on %s" % (self.name, tuple(shape), dtype, self.device))
-        if not out.is_contiguous() or out.data_ptr() % 16:
-            raise RockError("%s: out must be contiguous and start on a 16-byte boundary" % self.name)
-        return out
 
-    def launch(self, prog, info, *tensors):
-        if info is not None:
-            info["kernels"] = [k.kernel_name for k in prog.kernels]
-            info["kernel_name"] = prog.kernel_name
-            info["perf_config"] = prog.perf_config
-        with prog.lock:
-            for k in prog.kernels:
-                k.launch(*tensors)
+def _result(name, out, shape, dtype, like):
+    """`out` checked, or a new tensor on `like`'s device."""
+    if out is None:
+        return like.new_empty(shape, dtype=dtype)
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
+        raise RockError("%s: out must be %s of %s on %s" % (name, tuple(shape), dtype, like.device))
+    if not out.is_contiguous() or out.data_ptr() & 15:
+        raise RockError("%s: out must be contiguous and start on a 16-byte boundary" % name)
+    return out
 
 
-def _check_scale_vector(name, what, t, count):
+def _launch_tokens(prog, info, *tensors):
+    if info is not None:
+        info["kernels"] = [k.kernel_name for k in prog.kernels]
+        info["kernel_name"] = prog.kernel_name
+        info["perf_config"] = prog.perf_config
+    with prog.lock:
+        for k in prog.kernels:
+            k.launch_checked(tensors)
+
+
+def _scale_vector(name, what, t, count):
     import torch
     if not _is_tensor(t) or t.dtype != torch.float32 or t.numel() != count:
         raise RockError("%s: %s must hold %d float32 elements" % (name, what, count))
@@ -984,18 +1005,16 @@ def quantize_tokens(x, *, out=None, scale_out=None, stream=None, info=None):
     and of no other, are NaN.  Returns (q [..., K] int8, scale [...] float32), written into `out` and `scale_out`
     where given."""
     import torch
+    name = "quantize_tokens"
     if x.dim() < 1 or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise RockError("quantize_tokens: x is [..., K] of f16, bf16 or f32")
-    cols = x.shape[-1]
-    with _TokenCall("quantize_tokens", stream, x=x, out=out, scale_out=scale_out) as call:
-        q = call.result(out, x.shape, torch.int8)
-        s = call.result(scale_out, x.shape[:-1], torch.float32)
+    with _on(name, x.device, stream):
+        q = _result(name, out, x.shape, torch.int8, x)
+        s = _result(name, scale_out, x.shape[:-1], torch.float32, x)
         if x.numel() == 0:
-            if s.numel():       # rows without elements: their largest magnitude is 0
-                s.zero_()
-            return q, s
-        prog = _token_plan("quantize_tokens", _dtype_name(x.dtype), ("m", x.numel() // cols), ("k", cols))
-        call.launch(prog, info, _dense(x), q, s)
+            return q, s.zero_()   # rows without elements: their largest magnitude is 0
+        cols = x.shape[-1]
+        _launch_tokens(_token_plan(name, _dtype_name(x.dtype), m=x.numel() // cols, k=cols), info, _dense(x), q, s)
     return q, s
 
 
@@ -1018,28 +1037,35 @@ def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, a
     if out_dtype not in ("f16", "bf16", "f32"):
         raise RockError("%s: out_dtype f16, bf16 or f32" % name)
     vector = _is_tensor(scale)
-    with _TokenCall(name, stream, a=a, b=b, token_scale=token_scale, scale=scale if vector else None, bias=bias, out=out) as call:
-        ts = _check_scale_vector(name, "token_scale", token_scale, M)
-        cs = _check_scale_vector(name, "scale", scale, N) if vector else None
-        bv = None if bias is None else _check_scale_vector(name, "bias", bias, N)
-        res = call.result(out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype))
+    _same_device(name, a, b=b, token_scale=token_scale, scale=scale if vector else None, bias=bias)
+    with _on(name, a.device, stream):
+        tensors = [_dense(a), _dense(b), None, None if bias is None else _scale_vector(name, "bias", bias, N),
+                   _scale_vector(name, "token_scale", token_scale, M)]
+        if vector:
+            tensors.append(_scale_vector(name, "scale", scale, N))
+        res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a)
         if M == 0:
             return res
-        prog = _token_plan("gemm", "i8", ("m", M), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
-                           ("out_datatype", out_dtype), ("token_scale_vector", "true"),
-                           ("scale_vector", "true" if vector else None),
-                           ("scale", None if vector or scale is None else "%.9g" % scale),
-                           ("zero_point", zero_point or None), ("bias", None if bias is None else "true"),
-                           ("activation", "clip" if clip is not None else "relu" if relu else activation),
-                           ("clip_min", None if clip is None else "%.9g" % clip[0]),
-                           ("clip_max", None if clip is None else "%.9g" % clip[1]), ("perf_config", perf_config))
-        call.launch(prog, info, _dense(a), _dense(b), res, bv, ts, *([cs] if vector else []))
+        lo, hi = (None, None) if clip is None else (float(clip[0]), float(clip[1]))
+        prog = _token_plan("gemm", "i8", m=M, n=N, k=K, transB=bool(transB), out_datatype=out_dtype, token_scale_vector=True,
+                           scale_vector=vector, scale=None if vector or scale is None else float(scale),
+                           zero_point=int(zero_point) or None, bias=bias is not None,
+                           activation="clip" if clip is not None else "relu" if relu else activation, clip_min=lo,
+                           clip_max=hi, perf_config=perf_config)
+        _launch_tokens(prog, info, *tensors)
     return res
+
+
+def _check_offsets(name, offsets, E):
+    import torch
+    if E < 1:
+        raise RockError("%s: no experts" % name)
+    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != E + 1:
+        raise RockError("%s: offsets is int32 [E + 1], the first row of every expert and the end of the last" % name)
 
 
 def _grouped(name, rows, w, offsets, transB, cols_of_rows):
     """(groups, rows, N, K) of a grouped product, its operands checked; `cols_of_rows`: what `rows` holds per row."""
-    import torch
     if w.dim() != 3 or rows.dim() != 2 or rows.dtype != w.dtype:
         raise RockError("%s: rows [T, .] and weights [E, ., .] of one type" % name)
     E = w.shape[0]
@@ -1048,14 +1074,6 @@ def _grouped(name, rows, w, offsets, transB, cols_of_rows):
         raise RockError("%s: operand shapes do not match" % name)
     _check_offsets(name, offsets, E)
     return E, rows.shape[0], N, K
-
-
-def _check_offsets(name, offsets, E):
-    import torch
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != E + 1:
-        raise RockError("%s: offsets is int32 [E + 1], the first row of every expert and the end of the last" % name)
-    if E == 0:
-        raise RockError("%s: no experts" % name)
 
 
 def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=None, scale=None, out=None, stream=None,
@@ -1080,21 +1098,20 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
     if out_dtype not in ("f16", "bf16", "f32"):
         raise RockError("%s: out_dtype f16, bf16 or f32" % name)
     vector = _is_tensor(scale)
-    with _TokenCall(name, stream, x=x, w=w, offsets=offsets, token_scale=token_scale, scale=scale if vector else None,
-                    out=out) as call:
-        scales = []
+    _same_device(name, x, w=w, offsets=offsets, token_scale=token_scale, scale=scale if vector else None)
+    with _on(name, x.device, stream):
+        tensors = [_dense(x), _dense(w), None, _dense(offsets)]
         if token_scale is not None:
-            scales.append(_check_scale_vector(name, "token_scale", token_scale, T))
+            tensors.append(_scale_vector(name, "token_scale", token_scale, T))
         if vector:
-            scales.append(_check_scale_vector(name, "scale", scale, E * N))
-        res = call.result(out, (T, N), _torch_dtype(out_dtype))
+            tensors.append(_scale_vector(name, "scale", scale, E * N))
+        res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x)
         if T == 0 or N == 0:
             return res
-        prog = _token_plan("grouped_gemm", t, ("g", E), ("m", T), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
-                           ("out_datatype", out_dtype), ("token_scale_vector", None if token_scale is None else "true"),
-                           ("scale_vector", "true" if vector else None),
-                           ("scale", None if vector or scale is None else "%.9g" % scale), ("perf_config", perf_config))
-        call.launch(prog, info, _dense(x), _dense(w), res, _dense(offsets), *scales)
+        prog = _token_plan(name, t, g=E, m=T, n=N, k=K, transB=bool(transB), out_datatype=out_dtype,
+                           token_scale_vector=token_scale is not None, scale_vector=vector,
+                           scale=None if vector or scale is None else float(scale), perf_config=perf_config)
+        _launch_tokens(prog, info, *tensors)
     return res
 
 
@@ -1107,13 +1124,13 @@ def grouped_gemm_bwd_data(dout, w, offsets, *, transB=False, out=None, stream=No
     t = _dtype_name(dout.dtype)
     if t not in ("f32", "f16", "bf16"):
         raise RockError("%s: f16, bf16 or f32 operands" % name)
-    with _TokenCall(name, stream, dout=dout, w=w, offsets=offsets, out=out) as call:
-        res = call.result(out, (T, K), dout.dtype)
+    _same_device(name, dout, w=w, offsets=offsets)
+    with _on(name, dout.device, stream):
+        res = _result(name, out, (T, K), dout.dtype, dout)
         if T == 0 or K == 0:
             return res
-        prog = _token_plan(name, t, ("g", E), ("m", T), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
-                           ("perf_config", perf_config))
-        call.launch(prog, info, res, _dense(w), _dense(dout), _dense(offsets))
+        prog = _token_plan(name, t, g=E, m=T, n=N, k=K, transB=bool(transB), perf_config=perf_config)
+        _launch_tokens(prog, info, res, _dense(w), _dense(dout), _dense(offsets))
     return res
 
 
@@ -1124,18 +1141,18 @@ def grouped_gemm_bwd_weight(x, dout, offsets, *, transB=False, out=None, stream=
     name = "grouped_gemm_bwd_weight"
     if x.dim() != 2 or dout.dim() != 2 or x.shape[0] != dout.shape[0] or x.dtype != dout.dtype:
         raise RockError("%s: x [T, K] and dout [T, N] of one type" % name)
-    E, T, K, N = offsets.shape[0] - 1, x.shape[0], x.shape[1], dout.shape[1]
+    E, T, K, N = offsets.shape[0] - 1 if offsets.dim() == 1 else 0, x.shape[0], x.shape[1], dout.shape[1]
     _check_offsets(name, offsets, E)
     t = _dtype_name(x.dtype)
     if t not in ("f32", "f16", "bf16"):
         raise RockError("%s: f16, bf16 or f32 operands" % name)
-    with _TokenCall(name, stream, x=x, dout=dout, offsets=offsets, out=out) as call:
-        res = call.result(out, (E, N, K) if transB else (E, K, N), x.dtype)
+    _same_device(name, x, dout=dout, offsets=offsets)
+    with _on(name, x.device, stream):
+        res = _result(name, out, (E, N, K) if transB else (E, K, N), x.dtype, x)
         if res.numel() == 0:
             return res
         if T == 0:
             return res.zero_()
-        prog = _token_plan(name, t, ("g", E), ("m", T), ("n", N), ("k", K), ("transB", "true" if transB else "false"),
-                           ("perf_config", perf_config))
-        call.launch(prog, info, _dense(x), res, _dense(dout), _dense(offsets))
+        prog = _token_plan(name, t, g=E, m=T, n=N, k=K, transB=bool(transB), perf_config=perf_config)
+        _launch_tokens(prog, info, _dense(x), res, _dense(dout), _dense(offsets))
     return res

@@ -16,6 +16,29 @@ struct TokenTile {
 const TokenTile kTokenTiles[] = {
     {"_256x256", 256, 256, 2, 4, 1, 1.00f}, {"_128x128", 128, 128, 2, 2, 2, 0.75f}, {"_64x64", 64, 64, 2, 2, 4, 0.46f}};
 
+// Kernels for few rows (csrc/token_gemm.h): a block of eight waves per tile, K divided over the waves.
+const TokenTile kSkinnyTiles[] = {{"_16x16_skinny", 16, 16, 1, 8, 2, 0}, {"_16x32_skinny", 16, 32, 1, 8, 2, 0},
+                                  {"_32x16_skinny", 32, 16, 1, 8, 2, 0}, {"_32x32_skinny", 32, 32, 1, 8, 2, 0},
+                                  {"_64x32_skinny", 64, 32, 1, 8, 2, 0}};
+
+// The tile for a product of `rows` rows in `groups` groups, or NULL: too many rows per group.
+const TokenTile *pick_skinny_tile(int64_t rows, int64_t groups, int64_t cols, const OptMap &o) {
+  for (const TokenTile &t : kSkinnyTiles)
+    if (requested_tile_is(o, t.bm, t.bn))
+      return &t;
+  if (requested_tile_is(o, 64, 64) || !forced_tile(o).empty())
+    return nullptr;
+  const int64_t per_group = ceil_div(rows, std::min(rows, groups));
+  if (per_group > 64)
+    return nullptr;
+  const bool narrow = ceil_div(cols, 32) * std::min(rows, groups) < 2 * kNumCU;
+  if (per_group <= 16)
+    return &kSkinnyTiles[narrow ? 0 : 1];
+  if (per_group <= 32)
+    return &kSkinnyTiles[narrow ? 2 : 3];
+  return &kSkinnyTiles[4];
+}
+
 // The most row tiles of bm rows that `rows` rows in `groups` groups can make: every group that has a row may end in a
 // partial tile.
 int64_t row_tiles(int64_t rows, int64_t groups, int64_t bm) {
@@ -137,7 +160,15 @@ bool plan_token_gemm(Handle *h, const TokenProblem &q, int64_t cols, int64_t dep
   const bool b_ok = b_rows ? a_ok : al16(cols) && depth * cols * es + 256 * es < kMaxOff;
   const std::string name = std::string("rock_token_gemm_") + dtype_name(q.t);
   int64_t tiles_m;
-  if (a_ok && b_ok) {
+  if (const TokenTile *t = b_rows ? pick_skinny_tile(q.T, q.G, cols, o) : nullptr) {
+    tiles_m = row_tiles(q.T, q.G, t->bm);
+    p.tiles_n = ceil_div(cols, t->bn);
+    p.group_m = 8;
+    h->kernel_name = name + t->suffix;
+    h->perf_config = token_perf_string(t->bm, t->bn, 1, es);
+    if (!set_grid(h, tiles_m * p.tiles_n, 512, what))
+      return false;
+  } else if (a_ok && b_ok) {
     int64_t tiles[3];
     for (int i = 0; i < 3; ++i)
       tiles[i] = expected_row_tiles(q.T, q.G, kTokenTiles[i].bm) * ceil_div(cols, kTokenTiles[i].bn);
@@ -153,7 +184,7 @@ bool plan_token_gemm(Handle *h, const TokenProblem &q, int64_t cols, int64_t dep
     tiles_m = row_tiles(q.T, q.G, 64);
     p.tiles_n = ceil_div(cols, 64);
     p.group_m = 8;
-    h->kernel_name = name + "_64x64_generic";
+    h->kernel_name = name + "_64x64_any" + (b_rows ? "" : "_nn");
     h->perf_config = token_perf_string(64, 64, 2, es);
     if (!set_grid(h, tiles_m * p.tiles_n, 256, what))
       return false;
@@ -250,7 +281,7 @@ Handle *make_grouped_gemm(const OptMap &o) {
       h->kernel_name = name + t->suffix;
       h->perf_config = token_perf_string(bm, bn, t->waves_m, es);
     } else {
-      h->kernel_name = name + "_64x64_generic";
+      h->kernel_name = name + "_64x64_any";
       h->perf_config = token_perf_string(64, 64, 2, es);
     }
     p.tiles_m = ceil_div(M, bm);

@@ -280,17 +280,319 @@ __device__ __forceinline__ void token_gemm_body_dl(const void *A, const void *B,
                  });
 }
 
-template <int DT, int BM, int BN, int WM, int WN>
-__device__ __forceinline__ void token_gemm_body_generic(const void *A, const void *B, void *C, const void *bias,
-                                                        const int32_t *offsets, const float *token_scale,
-                                                        const float *channel_scale, const RockTokenGemmParams &tp) {
+// ---- operands of any alignment -----------------------------------------------------------------
+// Tiles of rows that are not whole 16-byte chunks: global -> registers -> LDS, the next K-step's loads in flight while
+// one is multiplied, LDS as in contraction_tile (rows of eight swizzled chunks).  Rows behind the last are read as the
+// last one -- their products are not stored -- and only the last K-step looks at where K ends.
+// K-contiguous rows: 16 bytes per load from wherever they start (global loads need no alignment).
+template <int DT, int ROWS, int NT> struct AnyRows {
+  using Gm = TileGeom<DT, ROWS, NT>;
+  const char *at[Gm::NCH]; // this lane's chunks at K-step 0
+  int k0, tid;
+  __device__ __forceinline__ void init(const void *base, int64_t row_stride, int64_t, int row0, int rows, int t) {
+    tid = t;
+    k0 = (t & 7) * Gm::EPC;
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i)
+      at[i] = (const char *)base + ((int64_t)min(row0 + (t >> 3) + i * Gm::ROW_STEP, rows - 1) * row_stride + k0) * Gm::ES;
+  }
+  template <bool TAIL> __device__ __forceinline__ void load(int kt, int K, v4i (&r)[Gm::NCH]) const {
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i) {
+      const char *src = at[i] + (int64_t)kt * kRowBytes;
+      if (!TAIL || K - (kt * Gm::BKE + k0) >= Gm::EPC) {
+        __builtin_memcpy(&r[i], src, 16);
+      } else {
+        const int left = K - (kt * Gm::BKE + k0);
+        r[i] = gather_chunk<DT>([&](int e) { return e < left ? load_elem<Gm::ES>(src, e) : 0u; });
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char *lds, const v4i (&r)[Gm::NCH]) const { store_tile<DT, ROWS, NT>(lds, r, tid); }
+};
+// K-major columns: neighbouring lanes take neighbouring columns, every load is one element of consecutive columns, and a
+// lane puts the elements of one column together to a chunk.
+template <int DT, int COLS, int NT> struct AnyCols {
+  using Gm = TileGeom<DT, COLS, NT>;
+  const char *at[Gm::NCH];
+  int64_t k_stride; // bytes between consecutive k
+  int tid;
+  __device__ __forceinline__ void init(const void *base, int64_t, int64_t ks, int col0, int cols, int t) {
+    tid = t;
+    k_stride = ks * Gm::ES;
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i) {
+      const int idx = t + i * NT;
+      at[i] = (const char *)base + (int64_t)min(col0 + idx % COLS, cols - 1) * Gm::ES + (idx / COLS) * Gm::EPC * k_stride;
+    }
+  }
+  template <bool TAIL> __device__ __forceinline__ void load(int kt, int K, v4i (&r)[Gm::NCH]) const {
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i) {
+      const char *src = at[i] + (int64_t)kt * Gm::BKE * k_stride;
+      const int left = K - (kt * Gm::BKE + (tid + i * NT) / COLS * Gm::EPC);
+      r[i] = gather_chunk<DT>([&](int e) { return !TAIL || e < left ? load_elem<Gm::ES>(src + e * k_stride, 0) : 0u; });
+    }
+  }
+  __device__ __forceinline__ void store(char *lds, const v4i (&r)[Gm::NCH]) const {
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i) {
+      const int idx = tid + i * NT, row = idx % COLS;
+      *(v4i *)(lds + row * kRowBytes + swizzle(row, idx / COLS) * kChunk) = r[i];
+    }
+  }
+};
+
+template <int DT, int BM, int BN, int WM, int WN, typename LoadA, typename LoadB, typename Params>
+__device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, const void *bias, const Params &p, int m0,
+                                         int n0) {
+  using Tr = MmaTraits<DT>;
+  using Acc = typename Tr::Acc;
+  constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32, NT = WM * WN * 64;
+  constexpr int STEPS = kChunksPerRow / (2 * Tr::CHUNKS), BKE = kRowBytes / Tr::ES;
+  constexpr int A_BYTES = BM * kRowBytes, STAGE = A_BYTES + BN * kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wm = wave % WM, wn = wave / WM, lrow = lane & 31, lgrp = lane >> 5;
+  LoadA la;
+  LoadB lb;
+  la.init(A, p.a_ms, p.a_ks, m0, p.M, tid);
+  lb.init(B, p.b_ns, p.b_ks, n0, p.N, tid);
+  v4i ra[LoadA::Gm::NCH], rb[LoadB::Gm::NCH];
+  Acc acc[MI][NI];
+#pragma unroll
+  for (int i = 0; i < MI; ++i)
+#pragma unroll
+    for (int j = 0; j < NI; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        acc[i][j][v] = 0;
+  const int nk = (p.K + BKE - 1) / BKE, whole = p.K / BKE;
+  auto fetch = [&](int kt) __attribute__((always_inline)) {
+    if (kt < whole) {
+      la.template load<false>(kt, p.K, ra);
+      lb.template load<false>(kt, p.K, rb);
+    } else {
+      la.template load<true>(kt, p.K, ra);
+      lb.template load<true>(kt, p.K, rb);
+    }
+  };
+  if (nk > 0) {
+    fetch(0);
+    la.store(lds, ra);
+    lb.store(lds + A_BYTES, rb);
+  }
+  __syncthreads();
+  for (int kt = 0; kt < nk; ++kt) {
+    const char *sa = lds + (kt & 1) * STAGE, *sb = sa + A_BYTES;
+    const bool more = kt + 1 < nk;
+    if (more)
+      fetch(kt + 1);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      Frag<DT> fb[NI];
+#pragma unroll
+      for (int j = 0; j < NI; ++j)
+        fb[j] = read_frag<DT>(sb, wn * WTN + j * 32 + lrow, s, lgrp);
+#pragma unroll
+      for (int i = 0; i < MI; ++i) {
+        const Frag<DT> fa = read_frag<DT>(sa, wm * WTM + i * 32 + lrow, s, lgrp);
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+          mma32x32<DT>(fb[j], fa, acc[i][j]);
+      }
+    }
+    if (more) {
+      char *da = lds + ((kt & 1) ^ 1) * STAGE;
+      la.store(da, ra);
+      lb.store(da + A_BYTES, rb);
+    }
+    __syncthreads();
+  }
+  using Acc4 = decltype(__builtin_shufflevector(acc[0][0], acc[0][0], 0, 1, 2, 3));
+  dispatch_tile_dtype<Tr::INT_ACC>(p, [&](auto od_const) __attribute__((always_inline)) {
+    constexpr int OD = decltype(od_const)::value;
+    direct_epilogue<Tr::INT_ACC, OD, MI, NI, Acc4, false>(acc, p, 0, C, bias, nullptr, m0 + wm * WTM + lrow,
+                                                          n0 + wn * WTN + lgrp * 4);
+  });
+}
+
+// B_COLS: the weights are stored [depth, columns]
+template <int DT, int BM, int BN, int WM, int WN, bool B_COLS>
+__device__ __forceinline__ void token_gemm_body_any(const void *A, const void *B, void *C, const void *bias,
+                                                    const int32_t *offsets, const float *token_scale,
+                                                    const float *channel_scale, const RockTokenGemmParams &tp) {
+  constexpr int NT = WM * WN * 64;
   GroupTile t;
   if (!locate_tile<BM>(offsets, tp.gemm, t))
     return;
   with_group<DT>(A, B, C, bias, token_scale, channel_scale, tp, t,
                  [&](const void *a, const void *b, void *c, const void *x, const auto &q) __attribute__((always_inline)) {
-                   contraction_tile<DT, BM, BN, WM, WN, LD_ROWS_GENERIC, LD_ROWS_GENERIC>(a, b, c, x, nullptr, q, 0,
-                                                                                          t.tm * BM, t.tn * BN);
+                   using LoadB = std::conditional_t<B_COLS, AnyCols<DT, BN, NT>, AnyRows<DT, BN, NT>>;
+                   any_tile<DT, BM, BN, WM, WN, AnyRows<DT, BM, NT>, LoadB>(a, b, c, x, q, t.tm * BM, t.tn * BN);
+                 });
+}
+
+// ---- few rows ------------------------------------------------------------------------------------
+// Products of a few token rows are bound by the weights' bytes, and what a tile kernel spends on filling LDS for one or
+// two K-steps at a time is latency.  Here a block takes 16 * CT columns and 16 * MT rows, its eight waves divide the
+// depth (64 bytes of every row in turn), weights and rows go straight from global memory into the operands of the 16 x 16
+// matrix instructions -- each weight is used by one wave only, so LDS has nothing to share -- with UNROLL K-steps of loads
+// in flight per wave, and the partial sums of the waves are added in wave order through LDS.
+template <int DT> struct SmallMma; // acc[n = 4 * (lane / 16) + v][m = lane % 16] += 16 bytes of k per lane and operand
+template <> struct SmallMma<MM_I8> {
+  using Acc = v4i;
+  static __device__ __forceinline__ Acc step(const v4i &w, const v4i &x, const Acc &c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0);
+  }
+};
+template <> struct SmallMma<MM_F16> {
+  using Acc = v4f;
+  static __device__ __forceinline__ Acc step(const v4i &w, const v4i &x, const Acc &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, w), __builtin_bit_cast(v8h, x), c, 0, 0, 0);
+  }
+};
+template <> struct SmallMma<MM_BF16> {
+  using Acc = v4f;
+  static __device__ __forceinline__ Acc step(const v4i &w, const v4i &x, const Acc &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, w), __builtin_bit_cast(v8bf, x), c, 0, 0, 0);
+  }
+};
+template <> struct SmallMma<MM_F32> {
+  using Acc = v4f;
+  static __device__ __forceinline__ Acc step(const v4i &w, const v4i &x, Acc c) {
+    const v4f a = __builtin_bit_cast(v4f, w), b = __builtin_bit_cast(v4f, x);
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[t], b[t], c, 0, 0, 0);
+    return c;
+  }
+};
+
+constexpr int kSkinnyWaves = 8;
+
+// 16 bytes of a row from element k on, zeros behind K
+template <int DT> __device__ __forceinline__ v4i row_chunk(const char *row, int k, int K) {
+  constexpr int ES = MmaTraits<DT>::ES, EPC = kChunk / ES;
+  v4i v = {0, 0, 0, 0};
+  const int left = K - k;
+  const char *src = row + (int64_t)k * ES;
+  if (left >= EPC)
+    __builtin_memcpy(&v, src, 16);
+  else if (left > 0)
+    v = gather_chunk<DT>([&](int e) { return e < left ? load_elem<ES>(src, e) : 0u; });
+  return v;
+}
+
+template <int DT, int MT, int CT, int UNROLL, typename Params>
+__device__ __forceinline__ void skinny_tile(const void *A, const void *B, void *C, const void *bias, const Params &p,
+                                            int m0, int n0) {
+  using Mma = SmallMma<DT>;
+  using Acc = typename Mma::Acc;
+  constexpr int ES = MmaTraits<DT>::ES, EPC = kChunk / ES, STEP = 64 / ES, W = kSkinnyWaves;
+  __shared__ __attribute__((aligned(16))) char lds[W * MT * CT * 64 * 16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int l16 = lane & 15, slice = lane >> 4;
+  const char *w[CT], *x[MT]; // rows behind the last are read as the last one: their results are not stored
+#pragma unroll
+  for (int j = 0; j < CT; ++j)
+    w[j] = (const char *)B + (int64_t)min(n0 + j * 16 + l16, p.N - 1) * p.b_ns * ES;
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+    x[i] = (const char *)A + (int64_t)min(m0 + i * 16 + l16, p.M - 1) * p.a_ms * ES;
+  Acc acc[MT][CT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+      acc[i][j] = Acc{0, 0, 0, 0};
+
+  const int steps = p.K / STEP; // whole K-steps: 64 bytes of every row
+  int s = wave;
+  auto batch = [&](auto n_const) __attribute__((always_inline)) {
+    constexpr int U = decltype(n_const)::value;
+    v4i wr[U][CT], xr[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t at = ((int64_t)(s + u * W) * 4 + slice) * kChunk;
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+        __builtin_memcpy(&wr[u][j], w[j] + at, 16);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        __builtin_memcpy(&xr[u][i], x[i] + at, 16);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < CT; ++j)
+          acc[i][j] = Mma::step(wr[u][j], xr[u][i], acc[i][j]);
+    s += U * W;
+  };
+  while (s + (UNROLL - 1) * W < steps)
+    batch(std::integral_constant<int, UNROLL>{});
+  if (UNROLL > 4 && s + 3 * W < steps)
+    batch(std::integral_constant<int, 4>{});
+  if (UNROLL > 2 && s + W < steps)
+    batch(std::integral_constant<int, 2>{});
+  if (s < steps)
+    batch(std::integral_constant<int, 1>{});
+  if (steps * STEP < p.K && wave == steps % W) { // what is left of K, less than a step
+    const int k = steps * STEP + slice * EPC;
+    v4i wr[CT], xr[MT];
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+      wr[j] = row_chunk<DT>(w[j], k, p.K);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      xr[i] = row_chunk<DT>(x[i], k, p.K);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < CT; ++j)
+        acc[i][j] = Mma::step(wr[j], xr[i], acc[i][j]);
+  }
+
+  Acc *sums = (Acc *)lds; // [wave][tile][lane]
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < CT; ++j)
+      sums[(wave * MT * CT + i * CT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  static_assert(MT * CT <= W, "a wave finishes one tile");
+  if (wave >= MT * CT)
+    return;
+  Acc sum = sums[wave * 64 + lane];
+#pragma unroll
+  for (int o = 1; o < W; ++o)
+    sum += sums[(o * MT * CT + wave) * 64 + lane];
+  const int m = m0 + wave / CT * 16 + l16, n = n0 + wave % CT * 16 + slice * 4;
+  if (m >= p.M || n >= p.N)
+    return;
+  int64_t row_off, n_stride;
+  bool vec_ok;
+  out_row_addr(p, 0, m, C, row_off, n_stride, vec_ok);
+  const auto rv = row_values(p, m);
+  dispatch_tile_dtype<MmaTraits<DT>::INT_ACC>(p, [&](auto od_const) __attribute__((always_inline)) {
+    constexpr int OD = decltype(od_const)::value;
+    const v4i raw = tile_convert4<MmaTraits<DT>::INT_ACC, OD>(sum, p, rv, bias, n);
+    store_packed4(raw, OutElemSize<OD>::value, C, row_off + n, n_stride, n, p.N, vec_ok && ((row_off + n) & 3) == 0);
+  });
+}
+
+template <int DT, int MT, int CT, int UNROLL>
+__device__ __forceinline__ void token_gemm_body_skinny(const void *A, const void *B, void *C, const void *bias,
+                                                       const int32_t *offsets, const float *token_scale,
+                                                       const float *channel_scale, const RockTokenGemmParams &tp) {
+  GroupTile t;
+  if (!locate_tile<MT * 16>(offsets, tp.gemm, t))
+    return;
+  with_group<DT>(A, B, C, bias, token_scale, channel_scale, tp, t,
+                 [&](const void *a, const void *b, void *c, const void *x, const auto &q) __attribute__((always_inline)) {
+                   skinny_tile<DT, MT, CT, UNROLL>(a, b, c, x, q, t.tm * MT * 16, t.tn * CT * 16);
                  });
 }
 
@@ -383,16 +685,16 @@ __device__ __forceinline__ void token_weight_body_dl(const void *A, const void *
 }
 
 template <int DT, int BM, int BN, int WM, int WN>
-__device__ __forceinline__ void token_weight_body_generic(const void *A, const void *B, void *C,
-                                                          const int32_t *offsets, const RockTokenWeightParams &wp) {
+__device__ __forceinline__ void token_weight_body_any(const void *A, const void *B, void *C, const int32_t *offsets,
+                                                      const RockTokenWeightParams &wp) {
+  constexpr int NT = WM * WN * 64;
   int g, tm, tn;
   decode_block(wp.gemm.tiles_m, wp.gemm.tiles_n, wp.gemm.G, wp.gemm.group_m, wp.gemm.xcd_remap, g, tm, tn);
   with_weight_group<DT>(A, B, C, offsets, wp, g,
                         [&](const void *a, const void *b, void *c, const TokenWeightTile &q)
                             __attribute__((always_inline)) {
-                              contraction_tile<DT, BM, BN, WM, WN, LD_ROWS_GENERIC, LD_ROWS_GENERIC>(
-                                  a, b, c, nullptr, nullptr, static_cast<const TokenTileParams &>(q), 0, tm * BM,
-                                  tn * BN);
+                              any_tile<DT, BM, BN, WM, WN, AnyCols<DT, BM, NT>, AnyCols<DT, BN, NT>>(
+                                  a, b, c, nullptr, q, tm * BM, tn * BN);
                             });
 }
 
@@ -411,17 +713,21 @@ __device__ __forceinline__ void token_weight_body_generic(const void *A, const v
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) { \
     rk::token_gemm_body_dl<ROCK_DT, BM, BN, WM, WN, LB>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
   }
-#define RK_TOKEN_GEMM(NAME, BM, BN, WM, WN)                                                           \
+#define RK_TOKEN_GEMM_ANY(NAME, BM, BN, WM, WN, B_COLS)                                               \
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) { \
-    rk::token_gemm_body_generic<ROCK_DT, BM, BN, WM, WN>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
+    rk::token_gemm_body_any<ROCK_DT, BM, BN, WM, WN, B_COLS>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
+  }
+#define RK_TOKEN_GEMM_SKINNY(NAME, MT, CT, UNROLL)                                                    \
+  extern "C" __global__ __launch_bounds__(512) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) {     \
+    rk::token_gemm_body_skinny<ROCK_DT, MT, CT, UNROLL>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
   }
 #define RK_TOKEN_WEIGHT_DL(NAME, BM, BN, WM, WN)                                                      \
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_WEIGHT_NAME(NAME)(               \
       const void *A, const void *B, void *C, const int32_t *offsets, RockTokenWeightParams p) {       \
     rk::token_weight_body_dl<ROCK_DT, BM, BN, WM, WN>(A, B, C, offsets, p);                           \
   }
-#define RK_TOKEN_WEIGHT(NAME, BM, BN, WM, WN)                                                         \
+#define RK_TOKEN_WEIGHT_ANY(NAME, BM, BN, WM, WN)                                                     \
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_WEIGHT_NAME(NAME)(               \
       const void *A, const void *B, void *C, const int32_t *offsets, RockTokenWeightParams p) {       \
-    rk::token_weight_body_generic<ROCK_DT, BM, BN, WM, WN>(A, B, C, offsets, p);                      \
+    rk::token_weight_body_any<ROCK_DT, BM, BN, WM, WN>(A, B, C, offsets, p);                      \
   }

@@ -75,6 +75,7 @@ def _no_timing(*args, **kwargs):
 
 
 api.RockKernel.launch = _launch
+api.RockKernel.launch_checked = lambda self, args: _launch(self, *args)
 api.RockKernel._pointer_array = _pointer_array
 api.RockKernel.benchmark = _no_timing
 api.mfma_rate = _no_timing

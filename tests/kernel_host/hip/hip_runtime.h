@@ -155,6 +155,18 @@ template <typename V, typename Acc> inline Acc hm_mfma_f8(V a, V b, Acc c, int f
 #define __builtin_amdgcn_mfma_i32_32x32x32_i8 hm_mfma_i8
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4 hm_mfma_f8
 
+// D (16 x 16) += A (16 x K) * B (K x 16): lane l holds its share of row (column) l % 16, the consecutive k starting at
+// (k per lane) * (l / 16); it receives column l % 16 of D, rows 4 * (l / 16) + v for its values v = 0..3.
+void hm_mfma_16x16(int type, const void *a, const void *b, int lane_bytes, void *acc4);
+template <int TYPE, int BYTES, typename V, typename Acc> inline Acc hm_mfma_small(V a, V b, Acc c, int, int, int) {
+  hm_mfma_16x16(TYPE, &a, &b, BYTES, &c);
+  return c;
+}
+#define __builtin_amdgcn_mfma_f32_16x16x32_f16 hm_mfma_small<HM_F16, 16>
+#define __builtin_amdgcn_mfma_f32_16x16x32_bf16 hm_mfma_small<HM_BF16, 16>
+#define __builtin_amdgcn_mfma_f32_16x16x4f32 hm_mfma_small<HM_F32, 4>
+#define __builtin_amdgcn_mfma_i32_16x16x64_i8 hm_mfma_small<HM_I8, 16>
+
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
 inline float __frcp_rn(float x) { return 1.0f / x; }
 inline float __expf(float x) { return expf(x); }

@@ -397,6 +397,25 @@ void hm_mfma_32x32(int type_a, int type_b, const void *a, const void *b, int lan
       ((float *)acc16)[v] = (float)((double)((float *)acc16)[v] + sum);
   }
 }
+void hm_mfma_16x16(int type, const void *a, const void *b, int lane_bytes, void *acc4) {
+  char *mine = my_slot();
+  std::memcpy(mine, a, lane_bytes);
+  std::memcpy(mine + 64, b, lane_bytes);
+  wait_as(kWaitWave);
+  const int l = lane_id(), per_lane = lane_bytes / elem_bytes(type);
+  for (int v = 0; v < 4; ++v) {
+    double sum = 0.0;
+    for (int slice = 0; slice < 4; ++slice) {
+      const char *ra = slot_of(4 * (l / 16) + v + 16 * slice), *cb = slot_of(l % 16 + 16 * slice) + 64;
+      for (int k = 0; k < per_lane; ++k)
+        sum += widen(type, ra, k) * widen(type, cb, k);
+    }
+    if (type == HM_I8)
+      ((int *)acc4)[v] = (int)((double)((int *)acc4)[v] + sum);
+    else
+      ((float *)acc4)[v] = (float)((double)((float *)acc4)[v] + sum);
+  }
+}
 
 extern "C" {
 // 0: loads into LDS land when issued; 1: not before the wait that covers them

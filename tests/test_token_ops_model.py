@@ -134,7 +134,7 @@ def test_int8_product_with_token_scales(model, rock, loads, shape, transB, extra
 # ---- products grouped by expert -----------------------------------------------------------------------------------
 # (groups' sizes, rows behind the last group, N, K): empty groups, one row, tiles that end inside a group, 70 groups
 GROUPS = [([5], 0, 24, 32), ([0, 3, 0, 64, 1, 0], 3, 40, 64), ([130, 0, 7], 5, 72, 48), ([0, 0], 4, 16, 32),
-          ([1] * 70 + [0, 9], 2, 16, 32), ([17, 40], 0, 33, 35), ([3, 66, 2], 1, 77, 64)]
+          ([1] * 70 + [0, 9], 2, 16, 32), ([17, 40], 0, 33, 35), ([3, 66, 2], 1, 77, 64), ([130, 0, 90], 2, 45, 37)]
 
 
 def _problem(sizes, tail, n, k, t, transB, seed=0):
@@ -223,6 +223,25 @@ def test_grouped_weight_gradient_every_tile(model, rock, loads, tile):
     dw = got[1][:w.nbytes].view(w.dtype).reshape(w.shape)
     for e, (a, b) in enumerate(bounds(offsets, T)):
         assert np.array_equal(dw[e].astype(np.float64), dout[a:b].astype(np.float64).T @ x[a:b].astype(np.float64)), e
+
+
+@pytest.mark.parametrize("tile", ["v2:16,16", "v2:16,32", "v2:32,16", "v2:32,32", "v2:64,32"])
+@pytest.mark.parametrize("t", ["f16", "f32", "i8"])
+@pytest.mark.parametrize("n,k", [(70, 35), (36, 1040), (33, 2501)])
+def test_grouped_product_every_kernel_for_few_rows(model, rock, tile, t, n, k):
+    """Depths below one K-step, of whole steps for every wave, and with a remainder behind them; columns that end
+    inside a tile; groups larger than the tile."""
+    sizes, tail = [1, 0, 17, 70, 3], 2
+    rng, T, E, offsets, x, w = _problem(sizes, tail, n, k, t, True)
+    extra = "-perf_config " + tile + (" -out_datatype f32" if t == "i8" else "")
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm", t, T, E, n, k, True, extra), {0: x, 1: w, 3: offsets})
+    assert not problems and tile[3:].replace(",", "x") + "_skinny" in names[0], (names, problems)
+    out = np.float32 if t == "i8" else _NUMPY[t]
+    res = got[2][:T * n * np.dtype(out).itemsize].view(out).reshape(T, n)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        want = x[a:b].astype(np.float64) @ w[e].T.astype(np.float64)
+        assert np.array_equal(res[a:b], want.astype(out)), e
+    assert (res[sum(sizes):].view(np.uint8) == 0xEE).all()
 
 
 @pytest.mark.parametrize("offsets", [[0, 5, 3, 9], [-4, 2, 100, 7], [4, 4, 4, 2], [9, 0, 0, 0], [2147483647] * 4, [-2147483648, 1, 1, 12]])
