@@ -109,6 +109,9 @@ def attention_kernels():
     return out
 
 
+# tiled kernels: K bytes per row and stage and number of stages of the products, of the weight gradient by element size
+TOKEN_TILES = {"_256x256": ((128, 2), {2: (128, 2), 4: (128, 2)}), "_128x128": ((128, 2), {2: (64, 2), 4: (128, 2)}),
+               "_64x64": ((128, 4), {2: (128, 2), 4: (128, 2)})}
 # kernels for few token rows: 16-row tiles, 16-column tiles, K-steps of loads in flight
 TOKEN_SKINNY = ((1, 1, 8), (1, 2, 8), (2, 1, 8), (2, 2, 4), (4, 2, 4))
 TOKEN_TYPES = {0: "f32", 1: "f16", 2: "bf16", 3: "i8"}
@@ -118,12 +121,14 @@ def token_kernels(type_code):
     """[(kernel name, macro invocation)] of the products of token rows (csrc/token_gemm.h) for one operand type."""
     t = TOKEN_TYPES[type_code]
     out = []
-    for tile in ("_256x256", "_128x128", "_64x64"):
+    for tile, (product, weight) in TOKEN_TILES.items():
         dims = "%d, %d, %d, %d" % TILES[tile]
-        out.append(("rock_token_gemm_%s%s_fast" % (t, tile), "RK_TOKEN_GEMM_DL(%s_fast, %s, %s)" % (tile, dims, ROWS)))
-        out.append(("rock_token_gemm_%s%s_fast_nn" % (t, tile), "RK_TOKEN_GEMM_DL(%s_fast_nn, %s, %s)" % (tile, dims, COLS)))
+        for suffix, loader in (("_fast", ROWS), ("_fast_nn", COLS)):
+            out.append(("rock_token_gemm_%s%s%s" % (t, tile, suffix),
+                        "RK_TOKEN_GEMM_DL(%s%s, %s, %s, %d, %d)" % ((tile, suffix, dims, loader) + product)))
         if t != "i8":
-            out.append(("rock_token_gemm_bwd_weight_%s%s" % (t, tile), "RK_TOKEN_WEIGHT_DL(%s, %s)" % (tile, dims)))
+            out.append(("rock_token_gemm_bwd_weight_%s%s" % (t, tile),
+                        "RK_TOKEN_WEIGHT_DL(%s, %s, %d, %d)" % ((tile, dims) + weight[4 if t == "f32" else 2])))
     for b_cols in (False, True):     # rows of any alignment
         name = "_64x64_any" + ("_nn" if b_cols else "")
         out.append(("rock_token_gemm_%s%s" % (t, name), "RK_TOKEN_GEMM_ANY(%s, 64, 64, 2, 2, %s)" % (name, str(b_cols).lower())))

@@ -561,6 +561,14 @@ __device__ __forceinline__ bool dl_epilogue_staged(const Params &p, const void *
   return out_rows_chunk_aligned(p, Cptr, out_elem_size(p.epi.out_dtype));
 }
 
+// Bytes of LDS a wave stages 32 rows of results in.  An output element takes up to four; the parameter blocks whose
+// results are all narrower say so (token_gemm.h).
+template <typename Params, int DT> struct MaxOutBytes : std::integral_constant<int, 4> {};
+template <int ES, int WTN> struct StagingBytes { // row-wise with 16 bytes of padding, or the transposed block
+  static constexpr int ROWS = 32 * (WTN * ES + 16), COLS = WTN * (32 * ES + (ES == 4 ? 0 : 16));
+  static constexpr int value = ROWS > COLS ? ROWS : COLS;
+};
+
 // Epilogue with a residual tensor or a transcendental activation.  Unrolled
 // over the accumulator registers, such an epilogue would repeat its loads,
 // address arithmetic and math routines for every group of four outputs (128
@@ -679,7 +687,7 @@ __device__ __forceinline__ void dl_epilogue_rich(typename MmaTraits<DT>::Acc (&a
                                                  int n_wave, char *lds, int wave, int lane, bool staged_ok) {
   using Tr = MmaTraits<DT>;
   constexpr int WTN = NI * 32;
-  constexpr int WBUF = 32 * (WTN * 4 + 16);
+  constexpr int WBUF = StagingBytes<4, WTN>::value;
   static_assert(NWAVES * WBUF <= LDS_BYTES, "staging buffers must fit in the operand stages");
   static_assert(NI * 4 * 1024 <= WBUF, "parked values must fit in the wave's staging buffer");
   using Acc4 = decltype(__builtin_shufflevector(acc[0][0], acc[0][0], 0, 1, 2, 3));
@@ -886,7 +894,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
       constexpr int ES = OutElemSize<OD>::value;
       constexpr int MP = 32 * ES + (ES == 4 ? 0 : 16); // bytes per channel row in LDS
       constexpr int VPR = 32 * ES / 16;                // 16-byte vectors per channel row
-      constexpr int WBUF = 32 * (WTN * 4 + 16);
+      constexpr int WBUF = StagingBytes<MaxOutBytes<Params, DT>::value, WTN>::value;
       static_assert(WTN * MP <= WBUF && NWAVES * WBUF <= LDS_BYTES, "transposed block must fit in the wave's region");
       char *wbuf = lds + wave * WBUF;
 #pragma unroll
@@ -941,7 +949,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
     constexpr int ES = OutElemSize<OD>::value;
     constexpr int ROWB = WTN * ES, PITCH = ROWB + 16;
     constexpr int LPR = ROWB / 16, RPI = 64 / LPR;
-    constexpr int WBUF = 32 * (WTN * 4 + 16);
+    constexpr int WBUF = StagingBytes<MaxOutBytes<Params, DT>::value, WTN>::value;
     static_assert(NWAVES * WBUF <= LDS_BYTES, "staging buffers must fit in the operand stages");
     char *wbuf = lds + wave * WBUF;
     const int rd_row = lane / LPR, rd_cb = (lane % LPR) * 16;
@@ -994,24 +1002,9 @@ __device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (
                                                    void *Cptr, const void *aux, int m_wave, int n_wave, char *lds,
                                                    int wave, int lane);
 
-// The output tile (g, m0.., n0..) by the calling block.
-template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int RB, int LDA, int LDB, bool RICH = false,
-          typename Params>
-__device__ __forceinline__ void contraction_tile_dl(const void *Aptr, const void *Bptr, void *Cptr,
-                                                    const void *aux, const void *res, const Params &p, int g, int m0,
-                                                    int n0) {
-  using Tr = MmaTraits<DT>;
-  using Acc = typename Tr::Acc;
-  constexpr int NW = WAVES_M * WAVES_N;
-  constexpr int WTM = BM / WAVES_M, WTN = BN / WAVES_N; // wave tile
-  constexpr int MI = WTM / 32, NI = WTN / 32;
-  constexpr int kDlStages = DlGeom<RB>::STAGES;
-  constexpr int STEPS = DlGeom<RB>::CHUNKS / (2 * Tr::CHUNKS); // MFMA K steps per stage
-  constexpr int A_BYTES = BM * RB, B_BYTES = BN * RB;
-  constexpr int STAGE = A_BYTES + B_BYTES;
-  constexpr int BKE = RB / Tr::ES;
-  static_assert(WTM % 32 == 0 && WTN % 32 == 0, "wave tile must be a multiple of 32");
-
+// How the LDS of a tile kernel is laid out.  With a K-major operand every stage is an LDS object of its own (below).
+template <int DT, int BM, int BN, int RB, int LDA, int LDB, int STAGES> struct DlLds {
+  static constexpr int STAGE = (BM + BN) * RB;
   // With a K-major operand the two stages are two LDS objects and the loop is
   // unrolled over them: the compiler puts an s_waitcnt vmcnt(0) in front of every
   // transposing LDS read that follows a load into LDS unless it can tell that
@@ -1020,13 +1013,34 @@ __device__ __forceinline__ void contraction_tile_dl(const void *Aptr, const void
   // in every K-step of the loading waves.
   // (Not for the 256x256 tile of the 8-bit float types: 128 accumulators and 96
   // fragment registers leave the unrolled loop no room and it spills.)
-  constexpr bool KM = (LDA == LD_COLS_FAST || LDB == LD_COLS_FAST || LDB == LD_CONV_COLS) &&
-                      !(Tr::CHUNKS == 2 && BM * BN >= 256 * 256);
-  static_assert(!KM || kDlStages == 2, "K-major operands: two stages, one LDS object each");
-  constexpr int WBUF = 32 * (WTN * 4 + 16); // the epilogue's staging region per wave
-  static_assert(!KM || (NW / 2) * WBUF <= STAGE, "half the waves stage their stores in each stage");
-  __shared__ __attribute__((aligned(1024))) char lds[KM ? STAGE : kDlStages * STAGE];
-  __shared__ __attribute__((aligned(1024))) char lds_hi[KM ? STAGE : 1024]; // K-major only
+  static constexpr bool KM = (LDA == LD_COLS_FAST || LDB == LD_COLS_FAST || LDB == LD_CONV_COLS) &&
+                             !(MmaTraits<DT>::CHUNKS == 2 && BM * BN >= 256 * 256);
+  static_assert(!KM || STAGES == 2 || STAGES == 4, "K-major operands: two or four stages, one LDS object each");
+  static constexpr int FIRST = KM ? STAGE : STAGES * STAGE; // bytes of the first object
+};
+
+// The output tile (g, m0.., n0..) by the calling block, in LDS of the caller: the first object and, with a K-major
+// operand, those of the other stages.
+template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int RB, int LDA, int LDB, bool RICH = false,
+          int kDlStages = DlGeom<RB>::STAGES, typename Params>
+__device__ __forceinline__ void contraction_tile_in(const void *Aptr, const void *Bptr, void *Cptr,
+                                                    const void *aux, const void *res, const Params &p, int g, int m0,
+                                                    int n0, char *lds, char *lds_hi, char *lds_2, char *lds_3) {
+  using Tr = MmaTraits<DT>;
+  using Acc = typename Tr::Acc;
+  constexpr int NW = WAVES_M * WAVES_N;
+  constexpr int WTM = BM / WAVES_M, WTN = BN / WAVES_N; // wave tile
+  constexpr int MI = WTM / 32, NI = WTN / 32;
+  constexpr int STEPS = DlGeom<RB>::CHUNKS / (2 * Tr::CHUNKS); // MFMA K steps per stage
+  constexpr int A_BYTES = BM * RB, B_BYTES = BN * RB;
+  constexpr int STAGE = A_BYTES + B_BYTES;
+  constexpr int BKE = RB / Tr::ES;
+  static_assert(WTM % 32 == 0 && WTN % 32 == 0, "wave tile must be a multiple of 32");
+
+  constexpr bool KM = DlLds<DT, BM, BN, RB, LDA, LDB, kDlStages>::KM;
+  constexpr int WBUF = StagingBytes<MaxOutBytes<Params, DT>::value, WTN>::value; // the epilogue's staging region per wave
+  constexpr int WPS = NW / kDlStages < 1 ? 1 : NW / kDlStages; // K-major: waves that stage their stores in one stage
+  static_assert(!KM || WPS * WBUF <= STAGE, "the waves' staging regions must fit in the stages");
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -1062,8 +1076,9 @@ __device__ __forceinline__ void contraction_tile_dl(const void *Aptr, const void
 #pragma unroll
   for (int s = 0; s < kDlStages - 1; ++s) {
     if (loader) {
-      la.issue(s, lds + s * STAGE);
-      lb.issue(s, lds + s * STAGE + A_BYTES);
+      char *stage = !KM || s == 0 ? lds + s * STAGE : s == 1 ? lds_hi : lds_2;
+      la.issue(s, stage);
+      lb.issue(s, stage + A_BYTES);
     }
   }
 
@@ -1138,7 +1153,21 @@ __device__ __forceinline__ void contraction_tile_dl(const void *Aptr, const void
       __builtin_amdgcn_sched_group_barrier(0x008, MI * NI, 0);
     }
   };
-  if constexpr (KM) {
+  if constexpr (KM && kDlStages == 4) {
+    int kt = 0;
+    for (; kt + 3 < nk; kt += 4) {
+      kstep(kt, lds, lds_3);
+      kstep(kt + 1, lds_hi, lds);
+      kstep(kt + 2, lds_2, lds_hi);
+      kstep(kt + 3, lds_3, lds_2);
+    }
+    if (kt < nk)
+      kstep(kt, lds, lds_3);
+    if (kt + 1 < nk)
+      kstep(kt + 1, lds_hi, lds);
+    if (kt + 2 < nk)
+      kstep(kt + 2, lds_2, lds_hi);
+  } else if constexpr (KM) {
     int kt = 0;
     for (; kt + 1 < nk; kt += 2) {
       kstep(kt, lds, lds_hi);
@@ -1155,14 +1184,30 @@ __device__ __forceinline__ void contraction_tile_dl(const void *Aptr, const void
 
   // the epilogue's staging region of wave w starts WBUF * w bytes behind the pointer it is given
   char *staging = lds;
-  if constexpr (KM)
-    staging = wave < NW / 2 ? lds : lds_hi - (NW / 2) * WBUF;
+  if constexpr (KM) {
+    const int in = wave / WPS;
+    staging = (in == 0 ? lds : in == 1 || kDlStages == 2 ? lds_hi : in == 2 ? lds_2 : lds_3) - in * WPS * WBUF;
+  }
   if constexpr (HasRowScales<Params>::value)
     row_scale_epilogue<DT, MI, NI, NW, kDlStages * STAGE>(acc, p, g, Cptr, aux, m0 + wm * WTM, n0 + wn * WTN, staging,
                                                           wave, lane);
   else
     dl_epilogue<DT, MI, NI, NW, kDlStages * STAGE, RICH>(acc, p, g, Cptr, aux, res, m0 + wm * WTM, n0 + wn * WTN,
                                                          staging, wave, lane);
+}
+
+template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int RB, int LDA, int LDB, bool RICH = false,
+          int STAGES = DlGeom<RB>::STAGES, typename Params>
+__device__ __forceinline__ void contraction_tile_dl(const void *Aptr, const void *Bptr, void *Cptr,
+                                                    const void *aux, const void *res, const Params &p, int g, int m0,
+                                                    int n0) {
+  using L = DlLds<DT, BM, BN, RB, LDA, LDB, STAGES>;
+  __shared__ __attribute__((aligned(1024))) char lds[L::FIRST];
+  __shared__ __attribute__((aligned(1024))) char lds_hi[L::KM ? L::STAGE : 1024]; // K-major only
+  __shared__ __attribute__((aligned(1024))) char lds_2[L::KM && STAGES == 4 ? L::STAGE : 1024];
+  __shared__ __attribute__((aligned(1024))) char lds_3[L::KM && STAGES == 4 ? L::STAGE : 1024];
+  contraction_tile_in<DT, BM, BN, WAVES_M, WAVES_N, RB, LDA, LDB, RICH, STAGES>(Aptr, Bptr, Cptr, aux, res, p, g, m0, n0,
+                                                                                lds, lds_hi, lds_2, lds_3);
 }
 
 template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int RB, int LDA, int LDB, bool RICH = false,

@@ -14,29 +14,35 @@ struct TokenTile {
   float efficiency; // as for the tiles of plan_gemm.cpp, whose kernels these are
 };
 const TokenTile kTokenTiles[] = {
-    {"_256x256", 256, 256, 2, 4, 1, 1.00f}, {"_128x128", 128, 128, 2, 2, 2, 0.75f}, {"_64x64", 64, 64, 2, 2, 4, 0.46f}};
+    {"_256x256", 256, 256, 2, 4, 1, 1.00f}, {"_128x128", 128, 128, 2, 2, 2, 0.75f}, {"_64x64", 64, 64, 2, 2, 2, 0.46f}};
 
 // Kernels for few rows (csrc/token_gemm.h): a block of eight waves per tile, K divided over the waves.
 const TokenTile kSkinnyTiles[] = {{"_16x16_skinny", 16, 16, 1, 8, 2, 0}, {"_16x32_skinny", 16, 32, 1, 8, 2, 0},
                                   {"_32x16_skinny", 32, 16, 1, 8, 2, 0}, {"_32x32_skinny", 32, 32, 1, 8, 2, 0},
                                   {"_64x32_skinny", 64, 32, 1, 8, 2, 0}};
 
-// The tile for a product of `rows` rows in `groups` groups, or NULL: too many rows per group.
-const TokenTile *pick_skinny_tile(int64_t rows, int64_t groups, int64_t cols, const OptMap &o) {
+// The tile for a product of `rows` rows in `groups` groups, or NULL: the tiled kernels.  Measured (i8, times in us in a
+// graph): the smallest tile whose blocks leave no compute unit two of them reads the fewest bytes per block, 16 rows of
+// 4096 x 4096 9.0 at 16 x 16 against 14.0 on 64 x 64 tiles, 64 rows of 1024 x 4096 7.1 against 13.7; with more blocks
+// than units the 64 x 64 tiles with three K-steps in flight stream as fast (16384 x 4096, one row: 19.7 against 19.2)
+// and take 64 rows at the same price, so only groups of one or two rows stay here (64 experts 2048 x 4096 at 64 rows: 71
+// against 79; at 256 rows 120 against 117).  `aligned`: the tiled kernels' 16-byte chunks fit; if not, the alternative
+// is the register-staged kernel, which these beat up to 64 rows per group.
+const TokenTile *pick_skinny_tile(int64_t rows, int64_t groups, int64_t cols, bool aligned, const OptMap &o) {
   for (const TokenTile &t : kSkinnyTiles)
     if (requested_tile_is(o, t.bm, t.bn))
       return &t;
-  if (requested_tile_is(o, 64, 64) || !forced_tile(o).empty())
+  if (o.count("perf_config"))
     return nullptr;
-  const int64_t per_group = ceil_div(rows, std::min(rows, groups));
-  if (per_group > 64)
-    return nullptr;
-  const bool narrow = ceil_div(cols, 32) * std::min(rows, groups) < 2 * kNumCU;
-  if (per_group <= 16)
-    return &kSkinnyTiles[narrow ? 0 : 1];
-  if (per_group <= 32)
-    return &kSkinnyTiles[narrow ? 2 : 3];
-  return &kSkinnyTiles[4];
+  const int64_t used = std::min(rows, groups), per_group = ceil_div(rows, used);
+  for (int i : {0, 1, 2, 3})
+    if (used * ceil_div(per_group, kSkinnyTiles[i].bm) * ceil_div(cols, kSkinnyTiles[i].bn) <= kNumCU)
+      return &kSkinnyTiles[i];
+  if (per_group <= (aligned ? 2 : 16))
+    return &kSkinnyTiles[1];
+  if (!aligned && per_group <= 64)
+    return &kSkinnyTiles[per_group <= 32 ? 3 : 4];
+  return nullptr;
 }
 
 // The most row tiles of bm rows that `rows` rows in `groups` groups can make: every group that has a row may end in a
@@ -55,10 +61,11 @@ int64_t expected_row_tiles(int64_t rows, int64_t groups, int64_t bm) {
 const TokenTile *pick_token_tile(int64_t tiles_of[3], const OptMap &o) {
   const TokenTile *best = nullptr;
   double best_cost = 0;
+  for (int i = 0; i < 3; ++i)
+    if (requested_tile_is(o, kTokenTiles[i].bm, kTokenTiles[i].bn))
+      return &kTokenTiles[i];
   for (int i = 0; i < 3; ++i) {
     const TokenTile &t = kTokenTiles[i];
-    if (requested_tile_is(o, t.bm, t.bn))
-      return &t;
     // rounds over the chip times the area of a tile, as pick_tile (plan_gemm.cpp) prices the same kernels
     const int64_t per_cu = (tiles_of[i] + kNumCU - 1) / kNumCU;
     double cost = (double)per_cu * t.bm * t.bn / t.efficiency;
@@ -160,7 +167,7 @@ bool plan_token_gemm(Handle *h, const TokenProblem &q, int64_t cols, int64_t dep
   const bool b_ok = b_rows ? a_ok : al16(cols) && depth * cols * es + 256 * es < kMaxOff;
   const std::string name = std::string("rock_token_gemm_") + dtype_name(q.t);
   int64_t tiles_m;
-  if (const TokenTile *t = b_rows ? pick_skinny_tile(q.T, q.G, cols, o) : nullptr) {
+  if (const TokenTile *t = b_rows ? pick_skinny_tile(q.T, q.G, cols, a_ok, o) : nullptr) {
     tiles_m = row_tiles(q.T, q.G, t->bm);
     p.tiles_n = ceil_div(cols, t->bn);
     p.group_m = 8;
@@ -178,7 +185,8 @@ bool plan_token_gemm(Handle *h, const TokenProblem &q, int64_t cols, int64_t dep
     p.group_m = t->bm >= 256 ? 4 : 8;
     h->kernel_name = name + t->suffix + "_fast" + (b_rows ? "" : "_nn");
     h->perf_config = token_perf_string(t->bm, t->bn, t->waves_m, es);
-    if (!set_grid(h, tiles_m * p.tiles_n, t->waves_m * t->waves_n * 64, what))
+    // (the last tiles of the largest kernel are cut into parts: up to one block per unit more, kUnits of token_gemm.h)
+    if (!set_grid(h, tiles_m * p.tiles_n + (t->bm == 256 ? kNumCU : 0), t->waves_m * t->waves_n * 64, what))
       return false;
   } else {
     tiles_m = row_tiles(q.T, q.G, 64);
@@ -287,8 +295,11 @@ Handle *make_grouped_gemm(const OptMap &o) {
     p.tiles_m = ceil_div(M, bm);
     p.tiles_n = ceil_div(N, bn);
     p.group_m = std::min(p.tiles_m, bm >= 256 ? 4 : 8);
-    const int64_t blocks = q.G * p.tiles_m * (int64_t)p.tiles_n;
-    p.xcd_remap = blocks >= 2 * kNumXCD ? 1 : 0;
+    int64_t blocks = q.G * p.tiles_m * (int64_t)p.tiles_n;
+    if (blocks > INT32_MAX)
+      blocks = -1;
+    else if (bm == 256)
+      blocks += kNumCU; // the last tiles in parts, as above
     if (!set_grid(h, blocks, threads, op.c_str())) {
       delete h;
       return nullptr;

@@ -151,6 +151,7 @@ __device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (
 // ---- which tile a block works on ---------------------------------------------------------
 struct GroupTile {
   int e, row0, rows, tm, tn; // group, its first row and row count, tile inside the group
+  int part, parts;           // which of how many parts of the tile
 };
 
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane * 4, v); }
@@ -185,49 +186,83 @@ __device__ __forceinline__ void scan_groups(const int32_t *offsets, int G, int M
   carry.tiles = __builtin_amdgcn_readfirstlane(lane_value(tiles_end, 63));
 }
 
-// The tile of this block; false: the block has none.  Uniform over the block: every wave computes the same.
-template <int BM>
-__device__ __forceinline__ bool locate_tile(const int32_t *offsets, const RockGemmParams &p, GroupTile &t) {
-  if (!offsets) {
-    int g;
-    decode_block(p.tiles_m, p.tiles_n, 1, p.group_m, p.xcd_remap, g, t.tm, t.tn);
-    t.e = 0;
-    t.row0 = 0;
-    t.rows = p.M;
+// The last tiles of a launch.  Tiles of 256 x 256 run one to a compute unit, so what is left after whole rounds over the
+// chip would keep a few units busy for a full round while the others idle: up to half a round of such tiles is cut
+// into halves (128 x 256), up to a quarter into quarters (128 x 128), which run side by side at the end.
+constexpr int kUnits = 256;
+__device__ __forceinline__ int tail_parts(int left) { return left * 4 <= kUnits ? 4 : left * 2 <= kUnits ? 2 : 1; }
+
+// Tile number and part of this block among `total` tiles; false: the block has none.  Consecutive tiles go to one XCD
+// (as decode_block does it) if `remap`.
+template <bool SPLIT>
+__device__ __forceinline__ bool block_tile(int total, bool remap, int &id, int &part, int &parts) {
+  auto spread = [&](int i, int n) {
+    const int per = n >> 3;
+    return remap && i < (per << 3) ? (i & 7) * per + (i >> 3) : i;
+  };
+  id = blockIdx.x;
+  part = 0;
+  parts = 1;
+  if constexpr (SPLIT) {
+    const int full = total & ~(kUnits - 1), left = total - full;
+    if (id >= full) {
+      parts = tail_parts(left);
+      if (id - full >= left * parts)
+        return false;
+      const int at = spread(id - full, left * parts);
+      id = full + at / parts;
+      part = at - at / parts * parts;
+    } else {
+      id = spread(id, full);
+    }
     return true;
   }
-  const int lane = threadIdx.x & 63;
-  const GroupScan first = {__builtin_amdgcn_readfirstlane(min(max(offsets[0], 0), p.M)), 0};
-  GroupScan all = first;
-  int start, end, tiles_end;
-  for (int base = 0; base < p.G; base += 64)
-    scan_groups<BM>(offsets, p.G, p.M, base, lane, all, start, end, tiles_end);
-  // consecutive tiles on one XCD, as decode_block does it, over the tiles there are
-  const int total = all.tiles * p.tiles_n; // at most the grid: the groups are disjoint
-  int id = blockIdx.x;
   if (id >= total)
     return false;
-  const int per = total >> 3;
-  if (id < (per << 3))
-    id = (id & 7) * per + (id >> 3);
-  const int tile_row = id / p.tiles_n; // the group is found by it: a group's tiles are whole rows of tiles
-  int base = 0;
-  if (p.G > 64) {
-    GroupScan seen = first;
-    for (;; base += 64) { // (ends: tile_row < all.tiles, which the last pass reaches)
-      scan_groups<BM>(offsets, p.G, p.M, base, lane, seen, start, end, tiles_end);
-      if (tile_row < seen.tiles || base + 64 >= p.G)
-        break;
-    }
+  id = spread(id, total);
+  return true;
+}
+
+// The tile of this block; false: the block has none.  Uniform over the block: every wave computes the same.
+template <int BM, bool SPLIT = false>
+__device__ __forceinline__ bool locate_tile(const int32_t *offsets, const RockGemmParams &p, GroupTile &t) {
+  const int lane = threadIdx.x & 63;
+  int start = 0, end = p.M, tiles_end = p.tiles_m, tile_rows = p.tiles_m;
+  GroupScan first = {0, 0};
+  if (offsets) {
+    first.end = __builtin_amdgcn_readfirstlane(min(max(offsets[0], 0), p.M));
+    GroupScan all = first;
+    for (int base = 0; base < p.G; base += 64)
+      scan_groups<BM>(offsets, p.G, p.M, base, lane, all, start, end, tiles_end);
+    tile_rows = all.tiles;
   }
-  const uint64_t beyond = __builtin_amdgcn_ballot_w64(tiles_end > tile_row);
-  const int at = beyond ? __builtin_ctzll(beyond) : 63;
-  t.e = base + at;
-  t.row0 = __builtin_amdgcn_readfirstlane(lane_value(start, at));
-  t.rows = __builtin_amdgcn_readfirstlane(lane_value(end, at)) - t.row0;
-  const int tiles_m = (t.rows + BM - 1) / BM;
-  const int group_first = __builtin_amdgcn_readfirstlane(lane_value(tiles_end, at)) - tiles_m; // tile rows before the group
-  const int in_group = id - group_first * p.tiles_n;
+  int id;
+  // (the tiles are at most the grid: the groups are disjoint)
+  if (!block_tile<SPLIT>(tile_rows * p.tiles_n, p.xcd_remap != 0, id, t.part, t.parts))
+    return false;
+  t.e = 0;
+  t.row0 = 0;
+  t.rows = p.M;
+  int tiles_m = p.tiles_m, in_group = id;
+  if (offsets) {
+    const int tile_row = id / p.tiles_n; // the group is found by it: a group's tiles are whole rows of tiles
+    int base = 0;
+    if (p.G > 64) {
+      GroupScan seen = first;
+      for (;; base += 64) { // (ends: tile_row < all.tiles, which the last pass reaches)
+        scan_groups<BM>(offsets, p.G, p.M, base, lane, seen, start, end, tiles_end);
+        if (tile_row < seen.tiles || base + 64 >= p.G)
+          break;
+      }
+    }
+    const uint64_t beyond = __builtin_amdgcn_ballot_w64(tiles_end > tile_row);
+    const int at = beyond ? __builtin_ctzll(beyond) : 63;
+    t.e = base + at;
+    t.row0 = __builtin_amdgcn_readfirstlane(lane_value(start, at));
+    t.rows = __builtin_amdgcn_readfirstlane(lane_value(end, at)) - t.row0;
+    tiles_m = (t.rows + BM - 1) / BM;
+    in_group -= (__builtin_amdgcn_readfirstlane(lane_value(tiles_end, at)) - tiles_m) * p.tiles_n;
+  }
   // inside the group: blocks of group_m tile rows, walked down the columns, so that neighbours share operand tiles
   const int group_sz = p.group_m * p.tiles_n;
   const int grp = in_group / group_sz;
@@ -266,24 +301,53 @@ __device__ __forceinline__ void with_group(const void *A, const void *B, void *C
   }
 }
 
-template <int DT, int BM, int BN, int WM, int WN, int LB>
+// One tile, or the block's part of it, in LDS that all of them share.
+template <int DT, int BM, int BN, int WM, int WN, int LA, int LB, int RB, int STAGES, typename Params>
+__device__ __forceinline__ void token_tile_dl(const void *a, const void *b, void *c, const void *bias, const Params &q,
+                                              int tm, int tn, int part, int parts) {
+  if constexpr (BM == 256) {
+    static_assert(BN == 256 && WM == 2 && WN == 4 && STAGES == 2, "the parts below");
+    using L = DlLds<DT, BM, BN, RB, LA, LB, 2>;
+    __shared__ __attribute__((aligned(1024))) char lds[L::FIRST];
+    __shared__ __attribute__((aligned(1024))) char lds_hi[L::KM ? L::STAGE : 1024];
+    const int m0 = tm * 256, n0 = tn * 256;
+    if (parts == 1) {
+      contraction_tile_in<DT, 256, 256, 2, 4, RB, LA, LB, false, 2>(a, b, c, bias, nullptr, q, 0, m0, n0, lds, lds_hi,
+                                                                    nullptr, nullptr);
+      return;
+    }
+    const int m = m0 + (part & 1) * 128, n = n0 + (part >> 1) * 128;
+    if (m >= q.M || n >= q.N)
+      return;
+    if (parts == 2)
+      contraction_tile_in<DT, 128, 256, 2, 4, RB, LA, LB, false, 2>(a, b, c, bias, nullptr, q, 0, m, n, lds, lds_hi,
+                                                                    nullptr, nullptr);
+    else
+      contraction_tile_in<DT, 128, 128, 2, 4, RB, LA, LB, false, 2>(a, b, c, bias, nullptr, q, 0, m, n, lds, lds_hi,
+                                                                    nullptr, nullptr);
+  } else {
+    contraction_tile_dl<DT, BM, BN, WM, WN, RB, LA, LB, false, STAGES>(a, b, c, bias, nullptr, q, 0, tm * BM, tn * BN);
+  }
+}
+
+template <int DT, int BM, int BN, int WM, int WN, int LB, int RB, int STAGES>
 __device__ __forceinline__ void token_gemm_body_dl(const void *A, const void *B, void *C, const void *bias,
                                                    const int32_t *offsets, const float *token_scale,
                                                    const float *channel_scale, const RockTokenGemmParams &tp) {
   GroupTile t;
-  if (!locate_tile<BM>(offsets, tp.gemm, t))
+  if (!locate_tile<BM, BM == 256>(offsets, tp.gemm, t))
     return;
   with_group<DT>(A, B, C, bias, token_scale, channel_scale, tp, t,
                  [&](const void *a, const void *b, void *c, const void *x, const auto &q) __attribute__((always_inline)) {
-                   contraction_tile_dl<DT, BM, BN, WM, WN, 128, LD_ROWS_FAST, LB>(a, b, c, x, nullptr, q, 0, t.tm * BM,
-                                                                                  t.tn * BN);
+                   token_tile_dl<DT, BM, BN, WM, WN, LD_ROWS_FAST, LB, RB, STAGES>(a, b, c, x, q, t.tm, t.tn, t.part,
+                                                                                   t.parts);
                  });
 }
 
 // ---- operands of any alignment -----------------------------------------------------------------
-// Tiles of rows that are not whole 16-byte chunks: global -> registers -> LDS, the next K-step's loads in flight while
-// one is multiplied, LDS as in contraction_tile (rows of eight swizzled chunks).  Rows behind the last are read as the
-// last one -- their products are not stored -- and only the last K-step looks at where K ends.
+// Tiles of rows that are not whole 16-byte chunks: global -> registers -> LDS, the loads of the next AHEAD K-steps in
+// flight while one is multiplied, LDS as in contraction_tile (rows of eight swizzled chunks).  Rows behind the last are
+// read as the last one -- their products are not stored -- and only the last K-step looks at where K ends.
 // K-contiguous rows: 16 bytes per load from wherever they start (global loads need no alignment).
 template <int DT, int ROWS, int NT> struct AnyRows {
   using Gm = TileGeom<DT, ROWS, NT>;
@@ -343,12 +407,12 @@ template <int DT, int COLS, int NT> struct AnyCols {
   }
 };
 
-template <int DT, int BM, int BN, int WM, int WN, typename LoadA, typename LoadB, typename Params>
+template <int DT, int BM, int BN, int WM, int WN, int AHEAD, typename LoadA, typename LoadB, typename Params>
 __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, const void *bias, const Params &p, int m0,
                                          int n0) {
   using Tr = MmaTraits<DT>;
   using Acc = typename Tr::Acc;
-  constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32, NT = WM * WN * 64;
+  constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32;
   constexpr int STEPS = kChunksPerRow / (2 * Tr::CHUNKS), BKE = kRowBytes / Tr::ES;
   constexpr int A_BYTES = BM * kRowBytes, STAGE = A_BYTES + BN * kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
@@ -358,7 +422,7 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
   LoadB lb;
   la.init(A, p.a_ms, p.a_ks, m0, p.M, tid);
   lb.init(B, p.b_ns, p.b_ks, n0, p.N, tid);
-  v4i ra[LoadA::Gm::NCH], rb[LoadB::Gm::NCH];
+  v4i ra[AHEAD][LoadA::Gm::NCH], rb[AHEAD][LoadB::Gm::NCH];
   Acc acc[MI][NI];
 #pragma unroll
   for (int i = 0; i < MI; ++i)
@@ -368,26 +432,25 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
       for (int v = 0; v < 16; ++v)
         acc[i][j][v] = 0;
   const int nk = (p.K + BKE - 1) / BKE, whole = p.K / BKE;
-  auto fetch = [&](int kt) __attribute__((always_inline)) {
+  auto fetch = [&](int kt, v4i(&a)[LoadA::Gm::NCH], v4i(&b)[LoadB::Gm::NCH]) __attribute__((always_inline)) {
     if (kt < whole) {
-      la.template load<false>(kt, p.K, ra);
-      lb.template load<false>(kt, p.K, rb);
-    } else {
-      la.template load<true>(kt, p.K, ra);
-      lb.template load<true>(kt, p.K, rb);
+      la.template load<false>(kt, p.K, a);
+      lb.template load<false>(kt, p.K, b);
+    } else if (kt < nk) {
+      la.template load<true>(kt, p.K, a);
+      lb.template load<true>(kt, p.K, b);
     }
   };
-  if (nk > 0) {
-    fetch(0);
-    la.store(lds, ra);
-    lb.store(lds + A_BYTES, rb);
-  }
-  __syncthreads();
-  for (int kt = 0; kt < nk; ++kt) {
-    const char *sa = lds + (kt & 1) * STAGE, *sb = sa + A_BYTES;
-    const bool more = kt + 1 < nk;
-    if (more)
-      fetch(kt + 1);
+#pragma unroll
+  for (int s = 0; s < AHEAD; ++s)
+    fetch(s, ra[s], rb[s]);
+  // K-step kt: its registers go to LDS, the loads of step kt + AHEAD take their place, then it is multiplied
+  auto kstep = [&](int kt, v4i(&a)[LoadA::Gm::NCH], v4i(&b)[LoadB::Gm::NCH]) __attribute__((always_inline)) {
+    char *sa = lds + (kt & 1) * STAGE, *sb = sa + A_BYTES;
+    la.store(sa, a);
+    lb.store(sb, b);
+    fetch(kt + AHEAD, a, b);
+    __syncthreads(); // step kt is in LDS, and everyone is done with step kt - 1: step kt + 1 may overwrite kt - 1
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       Frag<DT> fb[NI];
@@ -402,13 +465,13 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
           mma32x32<DT>(fb[j], fa, acc[i][j]);
       }
     }
-    if (more) {
-      char *da = lds + ((kt & 1) ^ 1) * STAGE;
-      la.store(da, ra);
-      lb.store(da + A_BYTES, rb);
-    }
-    __syncthreads();
-  }
+  };
+  for (int kt = 0; kt < nk; kt += AHEAD)
+    static_for<AHEAD>([&](auto sc) __attribute__((always_inline)) {
+      constexpr int s = decltype(sc)::value;
+      if (kt + s < nk)
+        kstep(kt + s, ra[s], rb[s]);
+    });
   using Acc4 = decltype(__builtin_shufflevector(acc[0][0], acc[0][0], 0, 1, 2, 3));
   dispatch_tile_dtype<Tr::INT_ACC>(p, [&](auto od_const) __attribute__((always_inline)) {
     constexpr int OD = decltype(od_const)::value;
@@ -429,7 +492,7 @@ __device__ __forceinline__ void token_gemm_body_any(const void *A, const void *B
   with_group<DT>(A, B, C, bias, token_scale, channel_scale, tp, t,
                  [&](const void *a, const void *b, void *c, const void *x, const auto &q) __attribute__((always_inline)) {
                    using LoadB = std::conditional_t<B_COLS, AnyCols<DT, BN, NT>, AnyRows<DT, BN, NT>>;
-                   any_tile<DT, BM, BN, WM, WN, AnyRows<DT, BM, NT>, LoadB>(a, b, c, x, q, t.tm * BM, t.tn * BN);
+                   any_tile<DT, BM, BN, WM, WN, B_COLS ? 2 : 3, AnyRows<DT, BM, NT>, LoadB>(a, b, c, x, q, t.tm * BM, t.tn * BN);
                  });
 }
 
@@ -597,8 +660,14 @@ __device__ __forceinline__ void token_gemm_body_skinny(const void *A, const void
 }
 
 // ---- weight gradient -----------------------------------------------------------------------
-// (its own type: the loaders below instead of those for operands within one 2 GiB window)
-struct TokenWeightTile : TokenTileParams {};
+// (its own type: the loaders below instead of those for operands within one 2 GiB window; results of the operands' type,
+// so that a wave's staging region takes half the LDS for 16-bit ones)
+template <int DT> struct TokenWeightTile : TokenTileParams {};
+template <int DT> struct MaxOutBytes<TokenWeightTile<DT>, DT> : std::integral_constant<int, MmaTraits<DT>::ES> {};
+template <bool INT_ACC, int DT, typename F>
+__device__ __forceinline__ void dispatch_tile_dtype(const TokenWeightTile<DT> &, F &&f) {
+  f(std::integral_constant<int, DT>{});
+}
 
 // ColsDl for a reduction over any number of rows: the buffer descriptor's base moves on with the K-steps in 64 bits
 // (scalar additions) and the lanes' offsets stay inside one stage.
@@ -645,13 +714,13 @@ template <int DT, int COLS, int NW, int RB> struct ColsLongDl {
   }
 };
 template <int DT, int ROWS, int NW, int RB, int KIND>
-__device__ __forceinline__ auto make_dl_a(const void *A, const TokenWeightTile &p, int, int m0, int wave, int lane) {
+__device__ __forceinline__ auto make_dl_a(const void *A, const TokenWeightTile<DT> &p, int, int m0, int wave, int lane) {
   ColsLongDl<DT, ROWS, NW, RB> l;
   l.init(A, p.a_ks, m0, p.M, p.K, wave, lane);
   return l;
 }
 template <int DT, int ROWS, int NW, int RB, int KIND>
-__device__ __forceinline__ auto make_dl_b(const void *B, const TokenWeightTile &p, int, int n0, int wave, int lane) {
+__device__ __forceinline__ auto make_dl_b(const void *B, const TokenWeightTile<DT> &p, int, int n0, int wave, int lane) {
   ColsLongDl<DT, ROWS, NW, RB> l;
   l.init(B, p.b_ks, n0, p.N, p.K, wave, lane);
   return l;
@@ -662,7 +731,7 @@ template <int DT, typename F>
 __device__ __forceinline__ void with_weight_group(const void *A, const void *B, void *C, const int32_t *offsets,
                                                   const RockTokenWeightParams &wp, int g, F &&f) {
   constexpr int ES = MmaTraits<DT>::ES;
-  TokenWeightTile q;
+  TokenWeightTile<DT> q;
   static_cast<RockGemmParams &>(q) = wp.gemm;
   const int lo = min(max(offsets[g], 0), q.K), hi = min(max(offsets[g + 1], lo), q.K);
   q.K = __builtin_amdgcn_readfirstlane(hi - lo);
@@ -671,16 +740,37 @@ __device__ __forceinline__ void with_weight_group(const void *A, const void *B, 
     (char *)C + (int64_t)g * q.c_gs * token_out_size(q.epi.out_dtype), q);
 }
 
-template <int DT, int BM, int BN, int WM, int WN>
+// Group by group: the tiles of one group go round the XCDs, so that a group with more rows than the others keeps all of
+// them busy longer and not the one that holds it.
+template <bool SPLIT>
+__device__ __forceinline__ bool locate_weight_tile(const RockGemmParams &p, GroupTile &t) {
+  int id;
+  const int tiles = p.tiles_m * p.tiles_n;
+  if (!block_tile<SPLIT>(tiles * p.G, false, id, t.part, t.parts))
+    return false;
+  t.e = id / tiles;
+  const int in_group = id - t.e * tiles;
+  const int group_sz = p.group_m * p.tiles_n;
+  const int grp = in_group / group_sz;
+  const int first_m = grp * p.group_m;
+  const int rows_here = min(p.tiles_m - first_m, p.group_m);
+  const int in_grp = in_group - grp * group_sz;
+  t.tm = first_m + in_grp % rows_here;
+  t.tn = in_grp / rows_here;
+  return true;
+}
+
+template <int DT, int BM, int BN, int WM, int WN, int RB, int STAGES>
 __device__ __forceinline__ void token_weight_body_dl(const void *A, const void *B, void *C, const int32_t *offsets,
                                                      const RockTokenWeightParams &wp) {
-  int g, tm, tn;
-  decode_block(wp.gemm.tiles_m, wp.gemm.tiles_n, wp.gemm.G, wp.gemm.group_m, wp.gemm.xcd_remap, g, tm, tn);
-  with_weight_group<DT>(A, B, C, offsets, wp, g,
-                        [&](const void *a, const void *b, void *c, const TokenWeightTile &q)
+  GroupTile t;
+  if (!locate_weight_tile<BM == 256>(wp.gemm, t))
+    return;
+  with_weight_group<DT>(A, B, C, offsets, wp, t.e,
+                        [&](const void *a, const void *b, void *c, const TokenWeightTile<DT> &q)
                             __attribute__((always_inline)) {
-                              contraction_tile_dl<DT, BM, BN, WM, WN, 128, LD_COLS_FAST, LD_COLS_FAST>(
-                                  a, b, c, nullptr, nullptr, q, 0, tm * BM, tn * BN);
+                              token_tile_dl<DT, BM, BN, WM, WN, LD_COLS_FAST, LD_COLS_FAST, RB, STAGES>(
+                                  a, b, c, nullptr, q, t.tm, t.tn, t.part, t.parts);
                             });
 }
 
@@ -688,13 +778,14 @@ template <int DT, int BM, int BN, int WM, int WN>
 __device__ __forceinline__ void token_weight_body_any(const void *A, const void *B, void *C, const int32_t *offsets,
                                                       const RockTokenWeightParams &wp) {
   constexpr int NT = WM * WN * 64;
-  int g, tm, tn;
-  decode_block(wp.gemm.tiles_m, wp.gemm.tiles_n, wp.gemm.G, wp.gemm.group_m, wp.gemm.xcd_remap, g, tm, tn);
-  with_weight_group<DT>(A, B, C, offsets, wp, g,
-                        [&](const void *a, const void *b, void *c, const TokenWeightTile &q)
+  GroupTile t;
+  if (!locate_weight_tile<false>(wp.gemm, t))
+    return;
+  with_weight_group<DT>(A, B, C, offsets, wp, t.e,
+                        [&](const void *a, const void *b, void *c, const TokenWeightTile<DT> &q)
                             __attribute__((always_inline)) {
-                              any_tile<DT, BM, BN, WM, WN, AnyCols<DT, BM, NT>, AnyCols<DT, BN, NT>>(
-                                  a, b, c, nullptr, q, tm * BM, tn * BN);
+                              any_tile<DT, BM, BN, WM, WN, 2, AnyCols<DT, BM, NT>, AnyCols<DT, BN, NT>>(
+                                  a, b, c, nullptr, q, t.tm * BM, t.tn * BN);
                             });
 }
 
@@ -709,9 +800,9 @@ __device__ __forceinline__ void token_weight_body_any(const void *A, const void 
   const void *A, const void *B, void *C, const void *bias, const int32_t *offsets,                    \
       const float *token_scale, const float *channel_scale, RockTokenGemmParams p
 
-#define RK_TOKEN_GEMM_DL(NAME, BM, BN, WM, WN, LB)                                                    \
+#define RK_TOKEN_GEMM_DL(NAME, BM, BN, WM, WN, LB, RB, STAGES)                                        \
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) { \
-    rk::token_gemm_body_dl<ROCK_DT, BM, BN, WM, WN, LB>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
+    rk::token_gemm_body_dl<ROCK_DT, BM, BN, WM, WN, LB, RB, STAGES>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
   }
 #define RK_TOKEN_GEMM_ANY(NAME, BM, BN, WM, WN, B_COLS)                                               \
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) { \
@@ -721,10 +812,10 @@ __device__ __forceinline__ void token_weight_body_any(const void *A, const void 
   extern "C" __global__ __launch_bounds__(512) void RK_TOKEN_GEMM_NAME(NAME)(RK_TOKEN_GEMM_ARGS) {     \
     rk::token_gemm_body_skinny<ROCK_DT, MT, CT, UNROLL>(A, B, C, bias, offsets, token_scale, channel_scale, p); \
   }
-#define RK_TOKEN_WEIGHT_DL(NAME, BM, BN, WM, WN)                                                      \
+#define RK_TOKEN_WEIGHT_DL(NAME, BM, BN, WM, WN, RB, STAGES)                                          \
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_WEIGHT_NAME(NAME)(               \
       const void *A, const void *B, void *C, const int32_t *offsets, RockTokenWeightParams p) {       \
-    rk::token_weight_body_dl<ROCK_DT, BM, BN, WM, WN>(A, B, C, offsets, p);                           \
+    rk::token_weight_body_dl<ROCK_DT, BM, BN, WM, WN, RB, STAGES>(A, B, C, offsets, p);                           \
   }
 #define RK_TOKEN_WEIGHT_ANY(NAME, BM, BN, WM, WN)                                                     \
   extern "C" __global__ __launch_bounds__(WM *WN * 64) void RK_TOKEN_WEIGHT_NAME(NAME)(               \

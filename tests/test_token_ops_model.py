@@ -225,6 +225,21 @@ def test_grouped_weight_gradient_every_tile(model, rock, loads, tile):
         assert np.array_equal(dw[e].astype(np.float64), dout[a:b].astype(np.float64).T @ x[a:b].astype(np.float64)), e
 
 
+@pytest.mark.parametrize("groups,n", [(300, 256), (350, 256), (200, 520)], ids=["quarters", "halves", "whole"])
+def test_last_tiles_in_parts(model, rock, groups, n):
+    """More 256 x 256 tiles than compute units: 256 whole ones, then 44 in quarters, 94 in halves; 600 tiles leave 88
+    in halves.  Groups of one to three rows, each a tile row of its own."""
+    sizes = [1 + g % 3 for g in range(groups)]
+    rng, T, E, offsets, x, w = _problem(sizes, 1, n, 16, "f16", True)
+    opts = _opts("grouped_gemm", "f16", T, E, n, 16, True, "-perf_config v2:256,256")
+    names, problems, got = run_plan(model, rock, opts, {0: x, 1: w, 3: offsets})
+    assert not problems and "256x256" in names[0], (names, problems)
+    res = got[2][:T * n * 2].view(np.float16).reshape(T, n)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        assert np.array_equal(res[a:b].astype(np.float64), x[a:b].astype(np.float64) @ w[e].T.astype(np.float64)), e
+    assert (res[sum(sizes):].view(np.uint8) == 0xEE).all()
+
+
 @pytest.mark.parametrize("tile", ["v2:16,16", "v2:16,32", "v2:32,16", "v2:32,32", "v2:64,32"])
 @pytest.mark.parametrize("t", ["f16", "f32", "i8"])
 @pytest.mark.parametrize("n,k", [(70, 35), (36, 1040), (33, 2501)])
