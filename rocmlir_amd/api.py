@@ -4,6 +4,7 @@ The option strings built here use the reference's own flag names
 (rocmlir-gen.cpp:90-561 for gemm / attention, ConvGenerator.cpp:492-661 for
 convolution), so a problem reads the same as on a rocmlir-gen command line.
 """
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -453,24 +454,31 @@ def _program(options):
     return p
 
 
-def _dtype_name(dt):
+_dtype_names, _torch_dtypes = {}, {}
+
+
+def _dtype_tables():
     import torch
-    names = {torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16",
-             torch.int8: "i8", torch.int32: "i32"}
+    names = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "i8": torch.int8, "i32": torch.int32}
     if hasattr(torch, "float8_e4m3fn"):
-        names[torch.float8_e4m3fn] = "fp8"
-        names[torch.float8_e5m2] = "bf8"
+        names["fp8"], names["bf8"] = torch.float8_e4m3fn, torch.float8_e5m2
+    _torch_dtypes.update(names)
+    _dtype_names.update({v: k for k, v in names.items()})
+
+
+def _dtype_name(dt):
+    if not _dtype_names:
+        _dtype_tables()
     try:
-        return names[dt]
+        return _dtype_names[dt]
     except KeyError:
         raise RockError("unsupported tensor dtype %s" % dt)
 
 
 def _torch_dtype(name):
-    import torch
-    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16,
-            "i8": torch.int8, "i32": torch.int32,
-            "fp8": torch.float8_e4m3fn, "bf8": torch.float8_e5m2}[name]
+    if not _torch_dtypes:
+        _dtype_tables()
+    return _torch_dtypes[name]
 
 
 def _is_tensor(x):
@@ -943,31 +951,25 @@ def _same_device(name, first, **others):
             raise RockError("%s: %s is on %s, the first operand on %s" % (name, what, t.device, first.device))
 
 
-class _on:
-    """Makes the operands' device the current one and `stream` (default: the device's current stream) torch's current
-    stream, so that copies and results made on the way are ordered with the kernels."""
+_here = contextlib.nullcontext()
 
-    def __init__(self, name, device, stream):
-        self._contexts = []
-        if device.type != "cuda":
-            return
-        import torch
-        if device.index != torch.cuda.current_device():
-            self._contexts.append(torch.cuda.device(device))
-        if stream is not None:
-            if not isinstance(stream, torch.cuda.Stream):
-                stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=device)
-            if stream.device != device:
-                raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, device))
-            self._contexts.append(torch.cuda.stream(stream))
 
-    def __enter__(self):
-        for c in self._contexts:
-            c.__enter__()
-
-    def __exit__(self, *exc):
-        for c in reversed(self._contexts):
-            c.__exit__(*exc)
+def _on(name, device, stream):
+    """A context that makes the operands' device the current one and `stream` (default: the device's current stream)
+    torch's current stream, so that copies and results made on the way are ordered with the kernels."""
+    import torch
+    if device.type != "cuda" or (stream is None and device.index == torch._C._cuda_getDevice()):
+        return _here
+    stack = contextlib.ExitStack()
+    stack.enter_context(torch.cuda.device(device))
+    if stream is not None:
+        if not isinstance(stream, torch.cuda.Stream):
+            stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=device)
+        if stream.device != device:
+            stack.close()
+            raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, device))
+        stack.enter_context(torch.cuda.stream(stream))
+    return stack
 
 
 def _result(name, out, shape, dtype, like):
@@ -1006,15 +1008,16 @@ def quantize_tokens(x, *, out=None, scale_out=None, stream=None, info=None):
     where given."""
     import torch
     name = "quantize_tokens"
-    if x.dim() < 1 or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+    shape = x.shape
+    if not shape or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise RockError("quantize_tokens: x is [..., K] of f16, bf16 or f32")
     with _on(name, x.device, stream):
-        q = _result(name, out, x.shape, torch.int8, x)
-        s = _result(name, scale_out, x.shape[:-1], torch.float32, x)
-        if x.numel() == 0:
+        q = _result(name, out, shape, torch.int8, x)
+        s = _result(name, scale_out, shape[:-1], torch.float32, x)
+        count, cols = x.numel(), shape[-1]
+        if count == 0:
             return q, s.zero_()   # rows without elements: their largest magnitude is 0
-        cols = x.shape[-1]
-        _launch_tokens(_token_plan(name, _dtype_name(x.dtype), m=x.numel() // cols, k=cols), info, _dense(x), q, s)
+        _launch_tokens(_token_plan(name, _dtype_name(x.dtype), m=count // cols, k=cols), info, _dense(x), q, s)
     return q, s
 
 

@@ -569,6 +569,10 @@ template <int ES, int WTN> struct StagingBytes { // row-wise with 16 bytes of pa
   static constexpr int value = ROWS > COLS ? ROWS : COLS;
 };
 
+// Results whose rows may start anywhere (token_gemm.h): the staged store writes 16 bytes per lane all the same -- global
+// stores need no alignment -- and only the pieces that hold a row's end go element by element.
+template <typename Params> struct AnyRowStart : std::false_type {};
+
 // Epilogue with a residual tensor or a transcendental activation.  Unrolled
 // over the accumulator registers, such an epilogue would repeat its loads,
 // address arithmetic and math routines for every group of four outputs (128
@@ -855,6 +859,25 @@ __device__ __forceinline__ void dl_epilogue_rich(typename MmaTraits<DT>::Acc (&a
   });
 }
 
+// 16 bytes of a row from any address on, or as many elements as are left of it
+typedef int v4i_any __attribute__((ext_vector_type(4), aligned(1)));
+template <int ES> __device__ __forceinline__ void store_row_piece(char *dst, const v4i &d, int left) {
+  if (left >= 16 / ES) {
+    __builtin_nontemporal_store(d, (v4i_any *)dst);
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < 16 / ES; ++k)
+    if (k < left) {
+      if constexpr (ES == 4)
+        ((int *)dst)[k] = d[k];
+      else if constexpr (ES == 2)
+        ((uint16_t *)dst)[k] = (uint16_t)((uint32_t)d[k >> 1] >> (16 * (k & 1)));
+      else
+        dst[k] = (char)((uint32_t)d[k >> 2] >> (8 * (k & 3)));
+    }
+}
+
 // RICH kernels are separate instantiations (kernel name suffix "_e") so that
 // the plain kernels' register allocation is untouched by the rich path.
 template <int DT, int MI, int NI, int NWAVES, int LDS_BYTES, bool RICH = false, typename Params>
@@ -868,7 +891,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
   const int lrow = lane & 31, lgrp = lane >> 5;
   const RockEpilogue &e = p.epi;
   using Acc4 = decltype(__builtin_shufflevector(acc[0][0], acc[0][0], 0, 1, 2, 3));
-  const bool staged_ok = dl_epilogue_staged(p, Cptr);
+  const bool staged_ok = AnyRowStart<Params>::value || dl_epilogue_staged(p, Cptr);
   if constexpr (RICH) {
     __builtin_amdgcn_s_barrier(); // every wave is done reading the operand stages
     dl_epilogue_rich<DT, MI, NI, NWAVES, LDS_BYTES>(acc, p, g, Cptr, aux, res, m_wave, n_wave, lds, wave, lane,
@@ -984,6 +1007,10 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
           int64_t row_off, n_stride;
           bool vec_ok;
           out_row_addr(p, g, m, Cptr, row_off, n_stride, vec_ok);
+          if constexpr (AnyRowStart<Params>::value) {
+            store_row_piece<ES>((char *)Cptr + (row_off + n) * ES, d, p.N - n);
+            continue;
+          }
           // streaming hint: the kernel never reads its output back, and the burst of
           // whole-row stores that every block issues at the same moment drains faster
           __builtin_nontemporal_store(d, (v4i *)((char *)Cptr + (row_off + n) * ES));

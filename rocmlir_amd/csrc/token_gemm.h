@@ -25,6 +25,8 @@ __device__ __forceinline__ void dispatch_tile_dtype(const TokenTileParams &p, F 
   }
 }
 
+template <> struct AnyRowStart<TokenTileParams> : std::true_type {};
+
 // ---- scales per token and channel -----------------------------------------------------
 struct TokenScaleParams : TokenTileParams {
   const float *token_scale;   // of the tile's group: element m belongs to row m
@@ -88,7 +90,6 @@ __device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (
     b[k] = e.has_bias ? ((const float *)aux)[at] : 0.0f;
   }
   const float zero_point = (float)e.zero_point;
-  const bool vec_rows = out_rows_chunk_aligned(p, Cptr, out_elem_size(e.out_dtype)) && n + VEC <= p.N;
   __builtin_amdgcn_s_barrier(); // every wave is done reading the operand stages
   dispatch_tile_dtype<true>(p, [&](auto od_const) __attribute__((always_inline)) {
     constexpr int OD = decltype(od_const)::value, ES = OutElemSize<OD>::value;
@@ -125,22 +126,11 @@ __device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (
         if (m >= p.M)
           continue;
         char *dst = (char *)Cptr + ((int64_t)g * p.c_gs + (int64_t)m * p.c_ms + n) * ES;
-        if (vec_rows) {
-          if constexpr (ES == 4) {
-            *(v4i *)dst = out[0];
-            *(v4i *)(dst + 16) = out[1];
-          } else {
-            __builtin_nontemporal_store(v4i{out[0][0], out[0][1], out[1][0], out[1][1]}, (v4i *)dst);
-          }
+        if constexpr (ES == 4) {
+          store_row_piece<4>(dst, out[0], p.N - n);
+          store_row_piece<4>(dst + 16, out[1], p.N - n - 4);
         } else {
-#pragma unroll
-          for (int k = 0; k < VEC; ++k)
-            if (n + k < p.N) {
-              if constexpr (ES == 4)
-                ((int *)dst)[k] = out[k >> 2][k & 3];
-              else
-                ((uint16_t *)dst)[k] = (uint16_t)((uint32_t)out[k >> 2][(k >> 1) & 1] >> (16 * (k & 1)));
-            }
+          store_row_piece<2>(dst, v4i{out[0][0], out[0][1], out[1][0], out[1][1]}, p.N - n);
         }
       }
       RK_WAVE_LDS_ORDER();
@@ -431,26 +421,33 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
 #pragma unroll
       for (int v = 0; v < 16; ++v)
         acc[i][j][v] = 0;
-  const int nk = (p.K + BKE - 1) / BKE, whole = p.K / BKE;
+  const int whole = p.K / BKE; // K-steps of 128 bytes; what is left of K is multiplied first
+  v4i ta[LoadA::Gm::NCH], tb[LoadB::Gm::NCH];
+  const bool tail = whole * BKE < p.K;
+  if (tail) {
+    la.template load<true>(whole, p.K, ta);
+    lb.template load<true>(whole, p.K, tb);
+  }
+  // (behind the last K-step it is loaded again, so that the loop needs no branch around its loads)
   auto fetch = [&](int kt, v4i(&a)[LoadA::Gm::NCH], v4i(&b)[LoadB::Gm::NCH]) __attribute__((always_inline)) {
-    if (kt < whole) {
-      la.template load<false>(kt, p.K, a);
-      lb.template load<false>(kt, p.K, b);
-    } else if (kt < nk) {
-      la.template load<true>(kt, p.K, a);
-      lb.template load<true>(kt, p.K, b);
-    }
+    la.template load<false>(min(kt, whole - 1), p.K, a);
+    lb.template load<false>(min(kt, whole - 1), p.K, b);
   };
+  if (whole > 0) {
 #pragma unroll
-  for (int s = 0; s < AHEAD; ++s)
-    fetch(s, ra[s], rb[s]);
-  // K-step kt: its registers go to LDS, the loads of step kt + AHEAD take their place, then it is multiplied
-  auto kstep = [&](int kt, v4i(&a)[LoadA::Gm::NCH], v4i(&b)[LoadB::Gm::NCH]) __attribute__((always_inline)) {
-    char *sa = lds + (kt & 1) * STAGE, *sb = sa + A_BYTES;
+    for (int s = 0; s < AHEAD; ++s)
+      fetch(s, ra[s], rb[s]);
+  }
+  // a K-step goes from its registers to LDS and is multiplied.  Two stages, one barrier: when everyone has passed the
+  // barrier of a step, everyone is done with the step before it, whose stage the next one overwrites.
+  int stage = 0;
+  auto multiply = [&](const v4i(&a)[LoadA::Gm::NCH], const v4i(&b)[LoadB::Gm::NCH], auto &&next)
+                      __attribute__((always_inline)) {
+    char *sa = lds + stage * STAGE, *sb = sa + A_BYTES;
     la.store(sa, a);
     lb.store(sb, b);
-    fetch(kt + AHEAD, a, b);
-    __syncthreads(); // step kt is in LDS, and everyone is done with step kt - 1: step kt + 1 may overwrite kt - 1
+    next();
+    __syncthreads();
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       Frag<DT> fb[NI];
@@ -465,12 +462,15 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
           mma32x32<DT>(fb[j], fa, acc[i][j]);
       }
     }
+    stage ^= 1;
   };
-  for (int kt = 0; kt < nk; kt += AHEAD)
+  if (tail)
+    multiply(ta, tb, [] {});
+  for (int kt = 0; kt < whole; kt += AHEAD)
     static_for<AHEAD>([&](auto sc) __attribute__((always_inline)) {
       constexpr int s = decltype(sc)::value;
-      if (kt + s < nk)
-        kstep(kt + s, ra[s], rb[s]);
+      if (kt + s < whole)
+        multiply(ra[s], rb[s], [&]() __attribute__((always_inline)) { fetch(kt + s + AHEAD, ra[s], rb[s]); });
     });
   using Acc4 = decltype(__builtin_shufflevector(acc[0][0], acc[0][0], 0, 1, 2, 3));
   dispatch_tile_dtype<Tr::INT_ACC>(p, [&](auto od_const) __attribute__((always_inline)) {
