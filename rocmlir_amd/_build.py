@@ -113,7 +113,7 @@ def attention_kernels():
 TOKEN_TILES = {"_256x256": ((128, 2), {2: (128, 2), 4: (128, 2)}), "_128x128": ((128, 2), {2: (64, 2), 4: (128, 2)}),
                "_64x64": ((128, 4), {2: (128, 2), 4: (128, 2)})}
 # kernels for few token rows: 16-row tiles, 16-column tiles, K-steps of loads in flight
-TOKEN_SKINNY = ((1, 1, 8), (1, 2, 8), (2, 1, 8), (2, 2, 4), (4, 2, 4))
+TOKEN_SKINNY = ((1, 1, 8), (1, 2, 8), (2, 1, 8), (2, 2, 4))
 TOKEN_TYPES = {0: "f32", 1: "f16", 2: "bf16", 3: "i8"}
 
 
@@ -129,9 +129,10 @@ def token_kernels(type_code):
         if t != "i8":
             out.append(("rock_token_gemm_bwd_weight_%s%s" % (t, tile),
                         "RK_TOKEN_WEIGHT_DL(%s, %s, %d, %d)" % ((tile, dims) + weight[4 if t == "f32" else 2])))
-    for b_cols in (False, True):     # rows of any alignment
-        name = "_64x64_any" + ("_nn" if b_cols else "")
-        out.append(("rock_token_gemm_%s%s" % (t, name), "RK_TOKEN_GEMM_ANY(%s, 64, 64, 2, 2, %s)" % (name, str(b_cols).lower())))
+    for tile in ("_128x128", "_64x64"):   # rows of any alignment
+        dims = "%d, %d, %d, %d" % TILES[tile]
+        for suffix, b_cols in (("_any", "false"), ("_any_nn", "true")):
+            out.append(("rock_token_gemm_%s%s%s" % (t, tile, suffix), "RK_TOKEN_GEMM_ANY(%s%s, %s, %s)" % (tile, suffix, dims, b_cols)))
     for mt, ct, unroll in TOKEN_SKINNY:
         name = "_%dx%d_skinny" % (16 * mt, 16 * ct)
         out.append(("rock_token_gemm_%s%s" % (t, name), "RK_TOKEN_GEMM_SKINNY(%s, %d, %d, %d)" % (name, mt, ct, unroll)))

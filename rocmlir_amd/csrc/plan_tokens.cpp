@@ -18,8 +18,7 @@ const TokenTile kTokenTiles[] = {
 
 // Kernels for few rows (csrc/token_gemm.h): a block of eight waves per tile, K divided over the waves.
 const TokenTile kSkinnyTiles[] = {{"_16x16_skinny", 16, 16, 1, 8, 2, 0}, {"_16x32_skinny", 16, 32, 1, 8, 2, 0},
-                                  {"_32x16_skinny", 32, 16, 1, 8, 2, 0}, {"_32x32_skinny", 32, 32, 1, 8, 2, 0},
-                                  {"_64x32_skinny", 64, 32, 1, 8, 2, 0}};
+                                  {"_32x16_skinny", 32, 16, 1, 8, 2, 0}, {"_32x32_skinny", 32, 32, 1, 8, 2, 0}};
 
 // The tile for a product of `rows` rows in `groups` groups, or NULL: the tiled kernels.  Measured (i8, times in us in a
 // graph): the smallest tile whose blocks leave no compute unit two of them reads the fewest bytes per block, 16 rows of
@@ -27,7 +26,7 @@ const TokenTile kSkinnyTiles[] = {{"_16x16_skinny", 16, 16, 1, 8, 2, 0}, {"_16x3
 // than units the 64 x 64 tiles with three K-steps in flight stream as fast (16384 x 4096, one row: 19.7 against 19.2)
 // and take 64 rows at the same price, so only groups of one or two rows stay here (64 experts 2048 x 4096 at 64 rows: 71
 // against 79; at 256 rows 120 against 117).  `aligned`: the tiled kernels' 16-byte chunks fit; if not, the alternative
-// is the register-staged kernel, which these beat up to 64 rows per group.
+// is the register-staged kernel, which is slower (f16, 20 experts 1001 x 515 at 51 rows each: 15 against 27 here).
 const TokenTile *pick_skinny_tile(int64_t rows, int64_t groups, int64_t cols, bool aligned, const OptMap &o) {
   for (const TokenTile &t : kSkinnyTiles)
     if (requested_tile_is(o, t.bm, t.bn))
@@ -40,8 +39,6 @@ const TokenTile *pick_skinny_tile(int64_t rows, int64_t groups, int64_t cols, bo
       return &kSkinnyTiles[i];
   if (per_group <= (aligned ? 2 : 16))
     return &kSkinnyTiles[1];
-  if (!aligned && per_group <= 64)
-    return &kSkinnyTiles[per_group <= 32 ? 3 : 4];
   return nullptr;
 }
 
@@ -189,11 +186,17 @@ bool plan_token_gemm(Handle *h, const TokenProblem &q, int64_t cols, int64_t dep
     if (!set_grid(h, tiles_m * p.tiles_n + (t->bm == 256 ? kNumCU : 0), t->waves_m * t->waves_n * 64, what))
       return false;
   } else {
-    tiles_m = row_tiles(q.T, q.G, 64);
-    p.tiles_n = ceil_div(cols, 64);
+    const TokenTile *t = nullptr; // 128 x 128 where they fill the chip twice, else 64 x 64
+    for (int i : {1, 2})
+      if (requested_tile_is(o, kTokenTiles[i].bm, kTokenTiles[i].bn))
+        t = &kTokenTiles[i];
+    if (!t)
+      t = &kTokenTiles[expected_row_tiles(q.T, q.G, 128) * ceil_div(cols, 128) >= 2 * kNumCU ? 1 : 2];
+    tiles_m = row_tiles(q.T, q.G, t->bm);
+    p.tiles_n = ceil_div(cols, t->bn);
     p.group_m = 8;
-    h->kernel_name = name + "_64x64_any" + (b_rows ? "" : "_nn");
-    h->perf_config = token_perf_string(64, 64, 2, es);
+    h->kernel_name = name + t->suffix + "_any" + (b_rows ? "" : "_nn");
+    h->perf_config = token_perf_string(t->bm, t->bn, t->waves_m, es);
     if (!set_grid(h, tiles_m * p.tiles_n, 256, what))
       return false;
   }

@@ -336,64 +336,139 @@ __device__ __forceinline__ void token_gemm_body_dl(const void *A, const void *B,
 
 // ---- operands of any alignment -----------------------------------------------------------------
 // Tiles of rows that are not whole 16-byte chunks: global -> registers -> LDS, the loads of the next AHEAD K-steps in
-// flight while one is multiplied, LDS as in contraction_tile (rows of eight swizzled chunks).  Rows behind the last are
-// read as the last one -- their products are not stored -- and only the last K-step looks at where K ends.
-// K-contiguous rows: 16 bytes per load from wherever they start (global loads need no alignment).
+// flight while one is multiplied, LDS as in the other tile kernels.  Every load is 16 bytes from wherever they start
+// (global loads need no alignment; measured they run at two thirds of the aligned rate): a chunk that would run
+// past the end of its row is loaded from that many elements further down and moved into place on its way to LDS, which
+// fills it up with zeros.  Rows behind the last are read as the last one, their products are not stored.
+// Rows shorter than a chunk are loaded element by element.
+__device__ __forceinline__ v4i move_down(const v4i &v, int bytes) { // byte i <- byte i + bytes, zeros from behind
+  typedef uint64_t v2u __attribute__((ext_vector_type(2)));
+  const v2u w = __builtin_bit_cast(v2u, v);
+  const int bits = bytes * 8;
+  v2u r;
+  r[0] = bits == 0 ? w[0] : bits < 64 ? (w[0] >> bits) | (w[1] << (64 - bits)) : bits < 128 ? w[1] >> (bits - 64) : 0;
+  r[1] = bits < 64 ? w[1] >> bits : 0;
+  return __builtin_bit_cast(v4i, r);
+}
+
+// The chunk of elements k .. of a row whose element k lies at src, as zeros from element K on.  Every lane loads all its
+// elements, those behind the last as the last: loads behind a test each would wait for each other, sixteen times the
+// latency of memory.
+template <int DT> __device__ __forceinline__ v4i tail_chunk(const char *src, int k, int K) {
+  constexpr int ES = MmaTraits<DT>::ES;
+  uint32_t v[kChunk / ES];
+#pragma unroll
+  for (int e = 0; e < kChunk / ES; ++e)
+    v[e] = load_elem<ES>(src, min(e, K - 1 - k));
+  return gather_chunk<DT>([&](int e) { return k + e < K ? v[e] : 0u; });
+}
+
+// K-contiguous rows
 template <int DT, int ROWS, int NT> struct AnyRows {
   using Gm = TileGeom<DT, ROWS, NT>;
-  const char *at[Gm::NCH]; // this lane's chunks at K-step 0
-  int k0, tid;
-  __device__ __forceinline__ void init(const void *base, int64_t row_stride, int64_t, int row0, int rows, int t) {
+  const char *row[Gm::NCH];
+  int k0, K, tid;
+  __device__ __forceinline__ void init(const void *base, int64_t row_stride, int64_t, int row0, int rows, int K_, int t) {
     tid = t;
+    K = K_;
     k0 = (t & 7) * Gm::EPC;
 #pragma unroll
     for (int i = 0; i < Gm::NCH; ++i)
-      at[i] = (const char *)base + ((int64_t)min(row0 + (t >> 3) + i * Gm::ROW_STEP, rows - 1) * row_stride + k0) * Gm::ES;
+      row[i] = (const char *)base + (int64_t)min(row0 + (t >> 3) + i * Gm::ROW_STEP, rows - 1) * row_stride * Gm::ES;
   }
-  template <bool TAIL> __device__ __forceinline__ void load(int kt, int K, v4i (&r)[Gm::NCH]) const {
+  static __device__ __forceinline__ bool narrow(int K, int) { return K < Gm::EPC; }
+  __device__ __forceinline__ void load(int kt, v4i (&r)[Gm::NCH]) const {
+    const int k = min(kt * Gm::BKE + k0, K - Gm::EPC);
 #pragma unroll
-    for (int i = 0; i < Gm::NCH; ++i) {
-      const char *src = at[i] + (int64_t)kt * kRowBytes;
-      if (!TAIL || K - (kt * Gm::BKE + k0) >= Gm::EPC) {
-        __builtin_memcpy(&r[i], src, 16);
-      } else {
-        const int left = K - (kt * Gm::BKE + k0);
-        r[i] = gather_chunk<DT>([&](int e) { return e < left ? load_elem<Gm::ES>(src, e) : 0u; });
-      }
-    }
+    for (int i = 0; i < Gm::NCH; ++i)
+      __builtin_memcpy(&r[i], row[i] + (int64_t)k * Gm::ES, 16);
   }
-  __device__ __forceinline__ void store(char *lds, const v4i (&r)[Gm::NCH]) const { store_tile<DT, ROWS, NT>(lds, r, tid); }
+  __device__ __forceinline__ void load_elements(int kt, v4i (&r)[Gm::NCH]) const {
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i)
+      r[i] = tail_chunk<DT>(row[i] + (int64_t)(kt * Gm::BKE + k0) * Gm::ES, kt * Gm::BKE + k0, K);
+  }
+  // last: K-step kt may hold the end of the rows
+  __device__ __forceinline__ void store(int kt, bool last, char *lds, v4i (&r)[Gm::NCH]) const {
+    if (last) {
+      const int k = kt * Gm::BKE + k0, beyond = k - min(k, K - Gm::EPC);
+#pragma unroll
+      for (int i = 0; i < Gm::NCH; ++i)
+        r[i] = move_down(r[i], min(beyond, Gm::EPC) * Gm::ES);
+    }
+    store_tile<DT, ROWS, NT>(lds, r, tid);
+  }
+  __device__ __forceinline__ void store_elements(char *lds, const v4i (&r)[Gm::NCH]) const { store_tile<DT, ROWS, NT>(lds, r, tid); }
+  static __device__ __forceinline__ Frag<DT> fragment(const char *lds, int block, int step, int lane) {
+    return read_frag<DT>(lds, block + (lane & 31), step, lane >> 5);
+  }
 };
-// K-major columns: neighbouring lanes take neighbouring columns, every load is one element of consecutive columns, and a
-// lane puts the elements of one column together to a chunk.
+
+// K-major columns: 16 bytes of consecutive columns of one k per load, LDS as ColsDl fills it (k-rows of swizzled chunks,
+// turned by the transposing reads)
 template <int DT, int COLS, int NT> struct AnyCols {
-  using Gm = TileGeom<DT, COLS, NT>;
-  const char *at[Gm::NCH];
-  int64_t k_stride; // bytes between consecutive k
-  int tid;
-  __device__ __forceinline__ void init(const void *base, int64_t, int64_t ks, int col0, int cols, int t) {
+  using Kg = KmGeom<DT, COLS, kRowBytes>;
+  struct Gm {
+    static constexpr int ES = Kg::ES, EPC = kChunk / ES, NCH = COLS * kRowBytes / kChunk / NT;
+    static_assert(COLS * kRowBytes % (kChunk * NT) == 0, "whole chunks per thread");
+  };
+  const char *base;
+  int64_t pitch; // bytes between consecutive k
+  int at[Gm::NCH], beyond[Gm::NCH]; // byte of a row where a lane's chunk is loaded from, elements it is moved down by
+  int cols, K, tid;
+  bool edge; // some lane's chunk is moved
+  __device__ __forceinline__ void init(const void *b, int64_t, int64_t ks, int col0, int c, int K_, int t) {
+    base = (const char *)b;
+    pitch = ks * Gm::ES;
+    cols = c;
+    K = K_;
     tid = t;
-    k_stride = ks * Gm::ES;
+    edge = col0 + COLS > c;
 #pragma unroll
     for (int i = 0; i < Gm::NCH; ++i) {
-      const int idx = t + i * NT;
-      at[i] = (const char *)base + (int64_t)min(col0 + idx % COLS, cols - 1) * Gm::ES + (idx / COLS) * Gm::EPC * k_stride;
+      const int col = col0 + (((t + i * NT) % Kg::CPR) ^ Kg::swz(krow(i))) * Gm::EPC, from = max(min(col, c - Gm::EPC), 0);
+      at[i] = from * Gm::ES;
+      beyond[i] = min(col - from, Gm::EPC);
     }
   }
-  template <bool TAIL> __device__ __forceinline__ void load(int kt, int K, v4i (&r)[Gm::NCH]) const {
+  __device__ __forceinline__ int krow(int i) const { return (tid + i * NT) / Kg::CPR; }
+  static __device__ __forceinline__ bool narrow(int, int cols) { return cols < Gm::EPC; }
+  __device__ __forceinline__ const char *row(int kt, int i) const {
+    return base + (int64_t)min(kt * Kg::KR + krow(i), K - 1) * pitch;
+  }
+  __device__ __forceinline__ void load(int kt, v4i (&r)[Gm::NCH]) const {
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i)
+      __builtin_memcpy(&r[i], row(kt, i) + at[i], 16);
+  }
+  __device__ __forceinline__ void load_elements(int kt, v4i (&r)[Gm::NCH]) const {
 #pragma unroll
     for (int i = 0; i < Gm::NCH; ++i) {
-      const char *src = at[i] + (int64_t)kt * Gm::BKE * k_stride;
-      const int left = K - (kt * Gm::BKE + (tid + i * NT) / COLS * Gm::EPC);
-      r[i] = gather_chunk<DT>([&](int e) { return !TAIL || e < left ? load_elem<Gm::ES>(src + e * k_stride, 0) : 0u; });
+      r[i] = tail_chunk<DT>(row(kt, i) + at[i] + beyond[i] * Gm::ES, at[i] / Gm::ES + beyond[i], cols);
+      if (kt * Kg::KR + krow(i) >= K)
+        r[i] = v4i{0, 0, 0, 0};
     }
   }
-  __device__ __forceinline__ void store(char *lds, const v4i (&r)[Gm::NCH]) const {
+  __device__ __forceinline__ void store(int kt, bool last, char *lds, v4i (&r)[Gm::NCH]) const {
+    if (edge) {
 #pragma unroll
-    for (int i = 0; i < Gm::NCH; ++i) {
-      const int idx = tid + i * NT, row = idx % COLS;
-      *(v4i *)(lds + row * kRowBytes + swizzle(row, idx / COLS) * kChunk) = r[i];
+      for (int i = 0; i < Gm::NCH; ++i)
+        r[i] = move_down(r[i], beyond[i] * Gm::ES);
     }
+    if (last) {
+#pragma unroll
+      for (int i = 0; i < Gm::NCH; ++i)
+        r[i] = kt * Kg::KR + krow(i) < K ? r[i] : v4i{0, 0, 0, 0};
+    }
+    store_elements(lds, r);
+  }
+  __device__ __forceinline__ void store_elements(char *lds, const v4i (&r)[Gm::NCH]) const {
+#pragma unroll
+    for (int i = 0; i < Gm::NCH; ++i)
+      *(v4i *)(lds + (tid + i * NT) * kChunk) = r[i];
+  }
+  static __device__ __forceinline__ Frag<DT> fragment(const char *lds, int block, int step, int lane) {
+    return dl_read_frag_km<DT, COLS, kRowBytes>(lds, block, step, lane);
   }
 };
 
@@ -402,16 +477,16 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
                                          int n0) {
   using Tr = MmaTraits<DT>;
   using Acc = typename Tr::Acc;
-  constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32;
+  constexpr int WTM = BM / WM, WTN = BN / WN, MI = WTM / 32, NI = WTN / 32, NW = WM * WN;
   constexpr int STEPS = kChunksPerRow / (2 * Tr::CHUNKS), BKE = kRowBytes / Tr::ES;
   constexpr int A_BYTES = BM * kRowBytes, STAGE = A_BYTES + BN * kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int wm = wave % WM, wn = wave / WM, lrow = lane & 31, lgrp = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wm = wave % WM, wn = wave / WM;
   LoadA la;
   LoadB lb;
-  la.init(A, p.a_ms, p.a_ks, m0, p.M, tid);
-  lb.init(B, p.b_ns, p.b_ks, n0, p.N, tid);
+  la.init(A, p.a_ms, p.a_ks, m0, p.M, p.K, tid);
+  lb.init(B, p.b_ns, p.b_ks, n0, p.N, p.K, tid);
   v4i ra[AHEAD][LoadA::Gm::NCH], rb[AHEAD][LoadB::Gm::NCH];
   Acc acc[MI][NI];
 #pragma unroll
@@ -421,42 +496,22 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
 #pragma unroll
       for (int v = 0; v < 16; ++v)
         acc[i][j][v] = 0;
-  const int whole = p.K / BKE; // K-steps of 128 bytes; what is left of K is multiplied first
-  v4i ta[LoadA::Gm::NCH], tb[LoadB::Gm::NCH];
-  const bool tail = whole * BKE < p.K;
-  if (tail) {
-    la.template load<true>(whole, p.K, ta);
-    lb.template load<true>(whole, p.K, tb);
-  }
-  // (behind the last K-step it is loaded again, so that the loop needs no branch around its loads)
-  auto fetch = [&](int kt, v4i(&a)[LoadA::Gm::NCH], v4i(&b)[LoadB::Gm::NCH]) __attribute__((always_inline)) {
-    la.template load<false>(min(kt, whole - 1), p.K, a);
-    lb.template load<false>(min(kt, whole - 1), p.K, b);
-  };
-  if (whole > 0) {
-#pragma unroll
-    for (int s = 0; s < AHEAD; ++s)
-      fetch(s, ra[s], rb[s]);
-  }
-  // a K-step goes from its registers to LDS and is multiplied.  Two stages, one barrier: when everyone has passed the
-  // barrier of a step, everyone is done with the step before it, whose stage the next one overwrites.
+  const int nk = (p.K + BKE - 1) / BKE;
   int stage = 0;
-  auto multiply = [&](const v4i(&a)[LoadA::Gm::NCH], const v4i(&b)[LoadB::Gm::NCH], auto &&next)
-                      __attribute__((always_inline)) {
-    char *sa = lds + stage * STAGE, *sb = sa + A_BYTES;
-    la.store(sa, a);
-    lb.store(sb, b);
-    next();
+  // Two stages, one barrier: when everyone has passed the barrier of a step, everyone is done with the step before it,
+  // whose stage the next one overwrites.
+  auto multiply = [&]() __attribute__((always_inline)) {
+    const char *sa = lds + stage * STAGE, *sb = sa + A_BYTES;
     __syncthreads();
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
       Frag<DT> fb[NI];
 #pragma unroll
       for (int j = 0; j < NI; ++j)
-        fb[j] = read_frag<DT>(sb, wn * WTN + j * 32 + lrow, s, lgrp);
+        fb[j] = LoadB::fragment(sb, wn * WTN + j * 32, s, lane);
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        const Frag<DT> fa = read_frag<DT>(sa, wm * WTM + i * 32 + lrow, s, lgrp);
+        const Frag<DT> fa = LoadA::fragment(sa, wm * WTM + i * 32, s, lane);
 #pragma unroll
         for (int j = 0; j < NI; ++j)
           mma32x32<DT>(fb[j], fa, acc[i][j]);
@@ -464,20 +519,47 @@ __device__ __forceinline__ void any_tile(const void *A, const void *B, void *C, 
     }
     stage ^= 1;
   };
-  if (tail)
-    multiply(ta, tb, [] {});
-  for (int kt = 0; kt < whole; kt += AHEAD)
+  if (LoadA::narrow(p.K, p.M) || LoadB::narrow(p.K, p.N)) {
+    for (int kt = 0; kt < nk; ++kt) {
+      la.load_elements(kt, ra[0]);
+      lb.load_elements(kt, rb[0]);
+      la.store_elements(lds + stage * STAGE, ra[0]);
+      lb.store_elements(lds + stage * STAGE + A_BYTES, rb[0]);
+      multiply();
+    }
+  } else if (nk > 0) {
+    // (behind the last K-step the last one is loaded again, so that the loop needs no branch around its loads)
+    auto fetch = [&](int kt, v4i(&a)[LoadA::Gm::NCH], v4i(&b)[LoadB::Gm::NCH]) __attribute__((always_inline)) {
+      la.load(min(kt, nk - 1), a);
+      lb.load(min(kt, nk - 1), b);
+    };
+    auto to_lds = [&](int kt, v4i(&a)[LoadA::Gm::NCH], v4i(&b)[LoadB::Gm::NCH]) __attribute__((always_inline)) {
+      la.store(kt, kt == nk - 1, lds + stage * STAGE, a);
+      lb.store(kt, kt == nk - 1, lds + stage * STAGE + A_BYTES, b);
+    };
+#pragma unroll
+    for (int s = 0; s < AHEAD; ++s)
+      fetch(s, ra[s], rb[s]);
+    int kt = 0;
+    for (; kt + AHEAD <= nk; kt += AHEAD)
+      static_for<AHEAD>([&](auto sc) __attribute__((always_inline)) {
+        constexpr int s = decltype(sc)::value;
+        to_lds(kt + s, ra[s], rb[s]);
+        fetch(kt + s + AHEAD, ra[s], rb[s]);
+        multiply();
+      });
     static_for<AHEAD>([&](auto sc) __attribute__((always_inline)) {
       constexpr int s = decltype(sc)::value;
-      if (kt + s < whole)
-        multiply(ra[s], rb[s], [&]() __attribute__((always_inline)) { fetch(kt + s + AHEAD, ra[s], rb[s]); });
+      if (kt + s < nk) {
+        to_lds(kt + s, ra[s], rb[s]);
+        multiply();
+      }
     });
-  using Acc4 = decltype(__builtin_shufflevector(acc[0][0], acc[0][0], 0, 1, 2, 3));
-  dispatch_tile_dtype<Tr::INT_ACC>(p, [&](auto od_const) __attribute__((always_inline)) {
-    constexpr int OD = decltype(od_const)::value;
-    direct_epilogue<Tr::INT_ACC, OD, MI, NI, Acc4, false>(acc, p, 0, C, bias, nullptr, m0 + wm * WTM + lrow,
-                                                          n0 + wn * WTN + lgrp * 4);
-  });
+  }
+  if constexpr (HasRowScales<Params>::value)
+    row_scale_epilogue<DT, MI, NI, NW, 2 * STAGE>(acc, p, 0, C, bias, m0 + wm * WTM, n0 + wn * WTN, lds, wave, lane);
+  else
+    dl_epilogue<DT, MI, NI, NW, 2 * STAGE>(acc, p, 0, C, bias, nullptr, m0 + wm * WTM, n0 + wn * WTN, lds, wave, lane);
 }
 
 // B_COLS: the weights are stored [depth, columns]
@@ -492,7 +574,7 @@ __device__ __forceinline__ void token_gemm_body_any(const void *A, const void *B
   with_group<DT>(A, B, C, bias, token_scale, channel_scale, tp, t,
                  [&](const void *a, const void *b, void *c, const void *x, const auto &q) __attribute__((always_inline)) {
                    using LoadB = std::conditional_t<B_COLS, AnyCols<DT, BN, NT>, AnyRows<DT, BN, NT>>;
-                   any_tile<DT, BM, BN, WM, WN, B_COLS ? 2 : 3, AnyRows<DT, BM, NT>, LoadB>(a, b, c, x, q, t.tm * BM, t.tn * BN);
+                   any_tile<DT, BM, BN, WM, WN, 3, AnyRows<DT, BM, NT>, LoadB>(a, b, c, x, q, t.tm * BM, t.tn * BN);
                  });
 }
 
@@ -533,19 +615,6 @@ template <> struct SmallMma<MM_F32> {
 };
 
 constexpr int kSkinnyWaves = 8;
-
-// 16 bytes of a row from element k on, zeros behind K
-template <int DT> __device__ __forceinline__ v4i row_chunk(const char *row, int k, int K) {
-  constexpr int ES = MmaTraits<DT>::ES, EPC = kChunk / ES;
-  v4i v = {0, 0, 0, 0};
-  const int left = K - k;
-  const char *src = row + (int64_t)k * ES;
-  if (left >= EPC)
-    __builtin_memcpy(&v, src, 16);
-  else if (left > 0)
-    v = gather_chunk<DT>([&](int e) { return e < left ? load_elem<ES>(src, e) : 0u; });
-  return v;
-}
 
 template <int DT, int MT, int CT, int UNROLL, typename Params>
 __device__ __forceinline__ void skinny_tile(const void *A, const void *B, void *C, const void *bias, const Params &p,
@@ -607,10 +676,10 @@ __device__ __forceinline__ void skinny_tile(const void *A, const void *B, void *
     v4i wr[CT], xr[MT];
 #pragma unroll
     for (int j = 0; j < CT; ++j)
-      wr[j] = row_chunk<DT>(w[j], k, p.K);
+      wr[j] = tail_chunk<DT>(w[j] + (int64_t)k * ES, k, p.K);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
-      xr[i] = row_chunk<DT>(x[i], k, p.K);
+      xr[i] = tail_chunk<DT>(x[i] + (int64_t)k * ES, k, p.K);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -663,6 +732,7 @@ __device__ __forceinline__ void token_gemm_body_skinny(const void *A, const void
 // (its own type: the loaders below instead of those for operands within one 2 GiB window; results of the operands' type,
 // so that a wave's staging region takes half the LDS for 16-bit ones)
 template <int DT> struct TokenWeightTile : TokenTileParams {};
+template <int DT> struct AnyRowStart<TokenWeightTile<DT>> : std::true_type {};
 template <int DT> struct MaxOutBytes<TokenWeightTile<DT>, DT> : std::integral_constant<int, MmaTraits<DT>::ES> {};
 template <bool INT_ACC, int DT, typename F>
 __device__ __forceinline__ void dispatch_tile_dtype(const TokenWeightTile<DT> &, F &&f) {
@@ -784,7 +854,7 @@ __device__ __forceinline__ void token_weight_body_any(const void *A, const void 
   with_weight_group<DT>(A, B, C, offsets, wp, t.e,
                         [&](const void *a, const void *b, void *c, const TokenWeightTile<DT> &q)
                             __attribute__((always_inline)) {
-                              any_tile<DT, BM, BN, WM, WN, 2, AnyCols<DT, BM, NT>, AnyCols<DT, BN, NT>>(
+                              any_tile<DT, BM, BN, WM, WN, 3, AnyCols<DT, BM, NT>, AnyCols<DT, BN, NT>>(
                                   a, b, c, nullptr, q, t.tm * BM, t.tn * BN);
                             });
 }

@@ -144,7 +144,7 @@ CASES = [  # (rows per expert, rows behind the last, N, K)
     ([1], 0, 64, 64), ([7], 0, 100, 36), ([0, 5, 0, 1, 33, 0], 3, 130, 64), ([300, 0, 77, 128], 20, 264, 192),
     ([3] * 40 + [0] * 30 + [1] * 90, 5, 48, 80), ([0, 0, 0], 6, 32, 32), ([257, 255, 256], 1, 520, 1040),
     ([19, 45], 0, 33, 35), ([2, 1, 0, 9], 2, 768, 4096), ([64, 1], 0, 65, 72), ([1000], 0, 80, 16),
-    ([130, 0, 290], 2, 75, 133), ([90, 1, 200], 0, 300, 1002)]
+    ([130, 0, 290], 2, 75, 133), ([200, 0, 70], 1, 5, 3), ([1, 200], 0, 9, 131), ([90, 1, 200], 0, 300, 1002)]
 
 
 def _ids(c):
