@@ -133,11 +133,11 @@ def token_kernels(type_code):
         dims = "%d, %d, %d, %d" % TILES[tile]
         for suffix, b_cols in (("_any", "false"), ("_any_nn", "true")):
             out.append(("rock_token_gemm_%s%s%s" % (t, tile, suffix), "RK_TOKEN_GEMM_ANY(%s%s, %s, %s)" % (tile, suffix, dims, b_cols)))
+        if t != "i8":
+            out.append(("rock_token_gemm_bwd_weight_%s%s_any" % (t, tile), "RK_TOKEN_WEIGHT_ANY(%s_any, %s)" % (tile, dims)))
     for mt, ct, unroll in TOKEN_SKINNY:
         name = "_%dx%d_skinny" % (16 * mt, 16 * ct)
         out.append(("rock_token_gemm_%s%s" % (t, name), "RK_TOKEN_GEMM_SKINNY(%s, %d, %d, %d)" % (name, mt, ct, unroll)))
-    if t != "i8":
-        out.append(("rock_token_gemm_bwd_weight_%s_64x64_any" % t, "RK_TOKEN_WEIGHT_ANY(_64x64_any, 64, 64, 2, 2)"))
     return out
 
 

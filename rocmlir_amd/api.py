@@ -186,6 +186,7 @@ class RockKernel:
         ncall = C.c_int(0)
         L.rockamdGetPointerMap(self._h, C.byref(ncall), None, None, None)
         self.caller_pointers = ncall.value
+        self._pointers = C.c_void_p * ncall.value
 
     def __del__(self):
         h, self._h = getattr(self, "_h", None), None
@@ -327,8 +328,7 @@ class RockKernel:
     def launch_checked(self, args):
         """launch() on torch's current stream for a caller that has checked the tensors against the problem's sizes
         and made their device the current one: a call costs the host a third of launch()."""
-        import torch
-        arr = (C.c_void_p * len(args))()
+        arr = self._pointers()
         for i, a in enumerate(args):
             if a is not None:
                 if not a.is_cuda:
@@ -920,15 +920,23 @@ def conv2d_bwd_weight(inp, dout, *, fil_layout, in_layout, out_layout, batchsize
 # operators over the token rows of a language model (csrc/plan_tokens.cpp)
 # ---------------------------------------------------------------------------
 _token_plans = {}
+torch = None   # the module, once one of these operators has been called
 
 
-def _token_plan(operation, t, **options):
-    """The plan of a problem (options that are None or False are left out)."""
-    key = (operation, t) + tuple(options.items())
+def _load_torch():
+    global torch
+    import torch as module
+    torch = module
+
+
+def _token_plan(names, *values):
+    """The plan of a problem given as the names of its options (one string) and their values; None and False leave an
+    option out.  The first two are the operation and the operands' type."""
+    key = (names, values)
     p = _token_plans.get(key)
     if p is None:
-        text = "-operation %s -arch gfx950 -t %s" % (operation, t)
-        for k, v in options.items():
+        text = "-arch gfx950"
+        for k, v in zip(names.split(), values):
             if v is not None and v is not False:
                 text += " -%s %s" % (k, "true" if v is True else "%.9g" % v if isinstance(v, float) else v)
         p = RockProgram(text)
@@ -957,7 +965,6 @@ _here = contextlib.nullcontext()
 def _on(name, device, stream):
     """A context that makes the operands' device the current one and `stream` (default: the device's current stream)
     torch's current stream, so that copies and results made on the way are ordered with the kernels."""
-    import torch
     if device.type != "cuda" or (stream is None and device.index == torch._C._cuda_getDevice()):
         return _here
     stack = contextlib.ExitStack()
@@ -994,7 +1001,6 @@ def _launch_tokens(prog, info, *tensors):
 
 
 def _scale_vector(name, what, t, count):
-    import torch
     if not _is_tensor(t) or t.dtype != torch.float32 or t.numel() != count:
         raise RockError("%s: %s must hold %d float32 elements" % (name, what, count))
     return _dense(t)
@@ -1006,7 +1012,8 @@ def quantize_tokens(x, *, out=None, scale_out=None, stream=None, info=None):
     scale 0 and q = 0; a row that holds an infinity or a NaN has scale NaN and q = 0, so that products of this row,
     and of no other, are NaN.  Returns (q [..., K] int8, scale [...] float32), written into `out` and `scale_out`
     where given."""
-    import torch
+    if torch is None:
+        _load_torch()
     name = "quantize_tokens"
     shape = x.shape
     if not shape or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
@@ -1017,14 +1024,15 @@ def quantize_tokens(x, *, out=None, scale_out=None, stream=None, info=None):
         count, cols = x.numel(), shape[-1]
         if count == 0:
             return q, s.zero_()   # rows without elements: their largest magnitude is 0
-        _launch_tokens(_token_plan(name, _dtype_name(x.dtype), m=count // cols, k=cols), info, _dense(x), q, s)
+        _launch_tokens(_token_plan("operation t m k", name, _dtype_name(x.dtype), count // cols, cols), info, _dense(x), q, s)
     return q, s
 
 
 def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, activation, clip, out, perf_config, stream,
                        info, token_scale):
     """gemm() with a scale for each row of the result."""
-    import torch
+    if torch is None:
+        _load_torch()
     name = "gemm with token_scale"
     if a.dtype != torch.int8 or b.dtype != torch.int8:
         raise RockError("%s: int8 operands" % name)
@@ -1050,17 +1058,16 @@ def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, a
         if M == 0:
             return res
         lo, hi = (None, None) if clip is None else (float(clip[0]), float(clip[1]))
-        prog = _token_plan("gemm", "i8", m=M, n=N, k=K, transB=bool(transB), out_datatype=out_dtype, token_scale_vector=True,
-                           scale_vector=vector, scale=None if vector or scale is None else float(scale),
-                           zero_point=int(zero_point) or None, bias=bias is not None,
-                           activation="clip" if clip is not None else "relu" if relu else activation, clip_min=lo,
-                           clip_max=hi, perf_config=perf_config)
+        prog = _token_plan("operation t token_scale_vector m n k transB out_datatype scale_vector scale zero_point bias "
+                           "activation clip_min clip_max perf_config", "gemm", "i8", True, M, N, K, bool(transB), out_dtype,
+                           vector, None if vector or scale is None else float(scale), int(zero_point) or None,
+                           bias is not None, "clip" if clip is not None else "relu" if relu else activation, lo, hi,
+                           perf_config)
         _launch_tokens(prog, info, *tensors)
     return res
 
 
 def _check_offsets(name, offsets, E):
-    import torch
     if E < 1:
         raise RockError("%s: no experts" % name)
     if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != E + 1:
@@ -1088,7 +1095,8 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
     bf16 and f32 operands give a result of their type unless `out_dtype` names another of the three; int8 operands
     give sum * scale * token_scale as f16 (default), bf16 or f32, `token_scale` float32 [T], `scale` float32 [E, N] or
     a number (both optional)."""
-    import torch
+    if torch is None:
+        _load_torch()
     name = "grouped_gemm"
     E, T, N, K = _grouped(name, x, w, offsets, transB, "K")
     i8 = x.dtype == torch.int8
@@ -1111,9 +1119,9 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
         res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x)
         if T == 0 or N == 0:
             return res
-        prog = _token_plan(name, t, g=E, m=T, n=N, k=K, transB=bool(transB), out_datatype=out_dtype,
-                           token_scale_vector=token_scale is not None, scale_vector=vector,
-                           scale=None if vector or scale is None else float(scale), perf_config=perf_config)
+        prog = _token_plan("operation t g m n k transB out_datatype token_scale_vector scale_vector scale perf_config", name, t,
+                           E, T, N, K, bool(transB), out_dtype, token_scale is not None, vector,
+                           None if vector or scale is None else float(scale), perf_config)
         _launch_tokens(prog, info, *tensors)
     return res
 
@@ -1122,6 +1130,8 @@ def grouped_gemm_bwd_data(dout, w, offsets, *, transB=False, out=None, stream=No
     """Gradient of grouped_gemm() with respect to x: rows of `dout` [T, N] times the transpose of their expert's
     weights (w and transB as given to grouped_gemm) -> [T, K] of dout's type, f16, bf16 or f32.  Rows of no expert
     are not written."""
+    if torch is None:
+        _load_torch()
     name = "grouped_gemm_bwd_data"
     E, T, N, K = _grouped(name, dout, w, offsets, transB, "N")
     t = _dtype_name(dout.dtype)
@@ -1132,7 +1142,7 @@ def grouped_gemm_bwd_data(dout, w, offsets, *, transB=False, out=None, stream=No
         res = _result(name, out, (T, K), dout.dtype, dout)
         if T == 0 or K == 0:
             return res
-        prog = _token_plan(name, t, g=E, m=T, n=N, k=K, transB=bool(transB), perf_config=perf_config)
+        prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
         _launch_tokens(prog, info, res, _dense(w), _dense(dout), _dense(offsets))
     return res
 
@@ -1141,6 +1151,8 @@ def grouped_gemm_bwd_weight(x, dout, offsets, *, transB=False, out=None, stream=
     """Gradient of grouped_gemm() with respect to w: for every expert the sum over its rows of x [T, K] and dout
     [T, N] -> [E, K, N] ([E, N, K] if transB) of their type, f16, bf16 or f32, summed in f32.  An expert without rows
     gets zeros."""
+    if torch is None:
+        _load_torch()
     name = "grouped_gemm_bwd_weight"
     if x.dim() != 2 or dout.dim() != 2 or x.shape[0] != dout.shape[0] or x.dtype != dout.dtype:
         raise RockError("%s: x [T, K] and dout [T, N] of one type" % name)
@@ -1156,6 +1168,6 @@ def grouped_gemm_bwd_weight(x, dout, offsets, *, transB=False, out=None, stream=
             return res
         if T == 0:
             return res.zero_()
-        prog = _token_plan(name, t, g=E, m=T, n=N, k=K, transB=bool(transB), perf_config=perf_config)
+        prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
         _launch_tokens(prog, info, _dense(x), res, _dense(dout), _dense(offsets))
     return res

@@ -10,15 +10,24 @@ namespace {
 
 struct TokenTile {
   const char *suffix;
-  int bm, bn, waves_m, waves_n, blocks_per_cu;
-  float efficiency; // as for the tiles of plan_gemm.cpp, whose kernels these are
+  int bm, bn, waves_m, waves_n;
+  double cost; // of one tile, the 256 x 256 tile's being 1
 };
-const TokenTile kTokenTiles[] = {
-    {"_256x256", 256, 256, 2, 4, 1, 1.00f}, {"_128x128", 128, 128, 2, 2, 2, 0.75f}, {"_64x64", 64, 64, 2, 2, 2, 0.46f}};
+// Measured with bf16 rows over 8 experts 2048 -> 4096 (us, rows 1024 / 2048 / 4096): 64 x 64 tiles 53 / 72 / 150 with
+// 4 / 8 / 16 of them per compute unit, 128 x 128 tiles 47 / 56 / 108 with 1 / 2 / 4, 256 x 256 tiles 49 / 51 / 92.
+const TokenTile kTokenTiles[] = {{"_256x256", 256, 256, 2, 4, 1.0}, {"_128x128", 128, 128, 2, 2, 0.47}, {"_64x64", 64, 64, 2, 2, 0.165}};
+
+// The time `tiles` tiles take, in tiles of 256 x 256.  The last of those run in parts (token_gemm.h: tail_parts).
+double tile_time(const TokenTile &t, int64_t tiles) {
+  if (t.bm < 256)
+    return (double)((tiles + kNumCU - 1) / kNumCU) * t.cost;
+  const int64_t left = tiles % kNumCU;
+  return (double)(tiles / kNumCU) + (left == 0 ? 0.0 : left * 4 <= kNumCU ? 0.4 : left * 2 <= kNumCU ? 0.6 : 1.0);
+}
 
 // Kernels for few rows (csrc/token_gemm.h): a block of eight waves per tile, K divided over the waves.
-const TokenTile kSkinnyTiles[] = {{"_16x16_skinny", 16, 16, 1, 8, 2, 0}, {"_16x32_skinny", 16, 32, 1, 8, 2, 0},
-                                  {"_32x16_skinny", 32, 16, 1, 8, 2, 0}, {"_32x32_skinny", 32, 32, 1, 8, 2, 0}};
+const TokenTile kSkinnyTiles[] = {{"_16x16_skinny", 16, 16, 1, 8, 0.0}, {"_16x32_skinny", 16, 32, 1, 8, 0.0},
+                                  {"_32x16_skinny", 32, 16, 1, 8, 0.0}, {"_32x32_skinny", 32, 32, 1, 8, 0.0}};
 
 // The tile for a product of `rows` rows in `groups` groups, or NULL: the tiled kernels.  Measured (i8, times in us in a
 // graph): the smallest tile whose blocks leave no compute unit two of them reads the fewest bytes per block, 16 rows of
@@ -55,25 +64,49 @@ int64_t expected_row_tiles(int64_t rows, int64_t groups, int64_t bm) {
   return used * ceil_div(ceil_div(rows, used), bm);
 }
 
-const TokenTile *pick_token_tile(int64_t tiles_of[3], const OptMap &o) {
-  const TokenTile *best = nullptr;
-  double best_cost = 0;
-  for (int i = 0; i < 3; ++i)
-    if (requested_tile_is(o, kTokenTiles[i].bm, kTokenTiles[i].bn))
-      return &kTokenTiles[i];
-  for (int i = 0; i < 3; ++i) {
-    const TokenTile &t = kTokenTiles[i];
-    // rounds over the chip times the area of a tile, as pick_tile (plan_gemm.cpp) prices the same kernels
-    const int64_t per_cu = (tiles_of[i] + kNumCU - 1) / kNumCU;
-    double cost = (double)per_cu * t.bm * t.bn / t.efficiency;
-    if (std::min<int64_t>(per_cu, t.blocks_per_cu) * t.waves_m * t.waves_n < 8)
-      cost /= 0.7;
-    if (!best || cost < best_cost) {
+const TokenTile *requested_tile(const OptMap &o) {
+  for (const TokenTile &t : kTokenTiles)
+    if (requested_tile_is(o, t.bm, t.bn))
+      return &t;
+  return nullptr;
+}
+
+// The tile with the least time for a product of `rows` rows in `groups` groups with `cols` columns.
+const TokenTile *pick_token_tile(int64_t rows, int64_t groups, int64_t cols, const OptMap &o) {
+  const TokenTile *best = requested_tile(o);
+  double best_time = 0;
+  if (best)
+    return best;
+  for (const TokenTile &t : kTokenTiles) {
+    const double time = tile_time(t, expected_row_tiles(rows, groups, t.bm) * ceil_div(cols, t.bn));
+    if (!best || time < best_time) {
       best = &t;
-      best_cost = cost;
+      best_time = time;
     }
   }
   return best;
+}
+
+// The tile of a weight gradient: `groups` results of M x N, each the sum over about `depth` rows.  The large tile pays
+// where the reduction is long (8 experts 4096 x 2048 bf16, us: 2048 rows each 242 against 294 on 128 x 128 and 566 on
+// 64 x 64; 256 rows 60 / 58 / 85), short ones are bound by their results and the latency of each tile, which the four
+// resident blocks of the 128 x 128 kernel hide (60 experts 1408 x 2048 at 83 rows 98 / 92 / 139; 64 experts 768 x 1024 at
+// 16 rows 30 / 23 / 33); few tiles want to be small (4 experts 512 x 512 at 1000 rows 15 / 18 / 14).  f32 results
+// stage in twice the LDS and the 128 x 128 kernel has two blocks (8 experts 1024 x 1024 at 250 rows 60 / 49 / 45).
+const TokenTile *pick_weight_tile(int64_t groups, int64_t M, int64_t N, int64_t depth, int es, const OptMap &o) {
+  if (const TokenTile *t = requested_tile(o))
+    return t;
+  auto tiles = [&](const TokenTile &t) { return groups * ceil_div(M, t.bm) * ceil_div(N, t.bn); };
+  if (depth >= 512 && tiles(kTokenTiles[0]) >= kNumCU / 2)
+    return &kTokenTiles[0];
+  return &kTokenTiles[tiles(kTokenTiles[1]) >= (es == 4 ? 4 : 1) * kNumCU ? 1 : 2];
+}
+
+// Operands of any alignment: 128 x 128 where `tiles` such tiles fill the chip twice (int8 4000 x 4096 x 2051: 94 us
+// against 129), else 64 x 64 (1001 x 2307 x 1283: 19 either way; 20 f16 experts 1001 x 515 at 51 rows 13 against 17).
+const TokenTile *pick_any_tile(int64_t tiles, const OptMap &o) {
+  const TokenTile *t = requested_tile(o);
+  return t && t->bm <= 128 ? t : &kTokenTiles[tiles >= 2 * kNumCU ? 1 : 2];
 }
 
 std::string token_perf_string(int bm, int bn, int waves_m, int es) {
@@ -173,10 +206,7 @@ bool plan_token_gemm(Handle *h, const TokenProblem &q, int64_t cols, int64_t dep
     if (!set_grid(h, tiles_m * p.tiles_n, 512, what))
       return false;
   } else if (a_ok && b_ok) {
-    int64_t tiles[3];
-    for (int i = 0; i < 3; ++i)
-      tiles[i] = expected_row_tiles(q.T, q.G, kTokenTiles[i].bm) * ceil_div(cols, kTokenTiles[i].bn);
-    const TokenTile *t = pick_token_tile(tiles, o);
+    const TokenTile *t = pick_token_tile(q.T, q.G, cols, o);
     tiles_m = row_tiles(q.T, q.G, t->bm);
     p.tiles_n = ceil_div(cols, t->bn);
     p.group_m = t->bm >= 256 ? 4 : 8;
@@ -186,12 +216,7 @@ bool plan_token_gemm(Handle *h, const TokenProblem &q, int64_t cols, int64_t dep
     if (!set_grid(h, tiles_m * p.tiles_n + (t->bm == 256 ? kNumCU : 0), t->waves_m * t->waves_n * 64, what))
       return false;
   } else {
-    const TokenTile *t = nullptr; // 128 x 128 where they fill the chip twice, else 64 x 64
-    for (int i : {1, 2})
-      if (requested_tile_is(o, kTokenTiles[i].bm, kTokenTiles[i].bn))
-        t = &kTokenTiles[i];
-    if (!t)
-      t = &kTokenTiles[expected_row_tiles(q.T, q.G, 128) * ceil_div(cols, 128) >= 2 * kNumCU ? 1 : 2];
+    const TokenTile *t = pick_any_tile(expected_row_tiles(q.T, q.G, 128) * ceil_div(cols, 128), o);
     tiles_m = row_tiles(q.T, q.G, t->bm);
     p.tiles_n = ceil_div(cols, t->bn);
     p.group_m = 8;
@@ -283,17 +308,16 @@ Handle *make_grouped_gemm(const OptMap &o) {
     const std::string name = std::string("rock_token_gemm_bwd_weight_") + dtype_name(q.t);
     int bm = 64, bn = 64, threads = 256;
     if (cols_ok(M) && cols_ok(N)) {
-      int64_t tiles[3];
-      for (int i = 0; i < 3; ++i)
-        tiles[i] = q.G * ceil_div(M, kTokenTiles[i].bm) * ceil_div(N, kTokenTiles[i].bn);
-      const TokenTile *t = pick_token_tile(tiles, o);
+      const TokenTile *t = pick_weight_tile(q.G, M, N, ceil_div(q.T, std::min(q.T, q.G)), es, o);
       bm = t->bm; bn = t->bn;
       threads = t->waves_m * t->waves_n * 64;
       h->kernel_name = name + t->suffix;
       h->perf_config = token_perf_string(bm, bn, t->waves_m, es);
     } else {
-      h->kernel_name = name + "_64x64_any";
-      h->perf_config = token_perf_string(64, 64, 2, es);
+      const TokenTile *t = pick_any_tile(q.G * ceil_div(M, 128) * ceil_div(N, 128), o);
+      bm = t->bm; bn = t->bn;
+      h->kernel_name = name + t->suffix + "_any";
+      h->perf_config = token_perf_string(bm, bn, t->waves_m, es);
     }
     p.tiles_m = ceil_div(M, bm);
     p.tiles_n = ceil_div(N, bn);

@@ -226,6 +226,41 @@ def test_grouped_weight_gradient_every_tile(model, rock, loads, tile):
         assert np.array_equal(dw[e].astype(np.float64), dout[a:b].astype(np.float64).T @ x[a:b].astype(np.float64)), e
 
 
+@pytest.mark.parametrize("tile", ["v2:128,128", "v2:64,64"])
+@pytest.mark.parametrize("t,transB", [("f16", True), ("f16", False), ("f32", False), ("i8", True)])
+@pytest.mark.parametrize("n,k", [(150, 77), (133, 261), (9, 200)])
+def test_every_tile_of_any_alignment(model, rock, loads, tile, t, transB, n, k):
+    """Rows that are no whole chunks: products, gradient of the rows, gradient of the weights; ends of rows inside a
+    chunk, a K-step of all zeros but one element, columns of one chunk."""
+    sizes, tail = [129, 0, 70, 1], 1
+    rng, T, E, offsets, x, w = _problem(sizes, tail, n, k, t, transB)
+    extra = "-perf_config " + tile + (" -out_datatype f32" if t == "i8" else "")
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm", t, T, E, n, k, transB, extra), {0: x, 1: w, 3: offsets})
+    es = np.dtype(_NUMPY[t]).itemsize
+    chunks = lambda c: c * es % 16 == 0   # noqa: E731
+    assert not problems and tile[3:].replace(",", "x") in names[0], (names, problems)
+    assert ("_any" in names[0]) == (not (chunks(k) and (transB or chunks(n)))), names
+    out = np.float32 if t == "i8" else _NUMPY[t]
+    res = got[2][:T * n * np.dtype(out).itemsize].view(out).reshape(T, n)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        want = x[a:b].astype(np.float64) @ (w[e].T if transB else w[e]).astype(np.float64)
+        assert np.array_equal(res[a:b], want.astype(out)), e
+    assert (res[sum(sizes):].view(np.uint8) == 0xEE).all()
+    if t == "i8":
+        return
+    dout = rng.integers(-3, 4, (T, n)).astype(_NUMPY[t])
+    dout[sum(sizes):] = np.nan
+    x[sum(sizes):] = np.nan
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_weight", t, T, E, n, k, transB, extra),
+                                    {0: x, 2: dout, 3: offsets})
+    assert not problems and tile[3:].replace(",", "x") in names[0], (names, problems)
+    assert ("_any" in names[0]) == (not (chunks(k) and chunks(n))), names
+    dw = got[1][:w.nbytes].view(w.dtype).reshape(w.shape)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        d64, x64 = dout[a:b].astype(np.float64), x[a:b].astype(np.float64)
+        assert np.array_equal(dw[e].astype(np.float64), d64.T @ x64 if transB else x64.T @ d64), e
+
+
 @pytest.mark.parametrize("groups,n", [(300, 256), (350, 256), (200, 520)], ids=["quarters", "halves", "whole"])
 def test_last_tiles_in_parts(model, rock, groups, n):
     """More 256 x 256 tiles than compute units: 256 whole ones, then 44 in quarters, 94 in halves; 600 tiles leave 88
