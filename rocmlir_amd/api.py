@@ -328,6 +328,8 @@ class RockKernel:
     def launch_checked(self, args):
         """launch() on torch's current stream for a caller that has checked the tensors against the problem's sizes
         and made their device the current one: a call costs the host a third of launch()."""
+        if torch is None:
+            _load_torch()
         arr = self._pointers()
         for i, a in enumerate(args):
             if a is not None:
