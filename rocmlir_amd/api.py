@@ -981,10 +981,15 @@ def _on(name, device, stream):
     return stack
 
 
-def _result(name, out, shape, dtype, like):
+def _result(name, out, shape, dtype, like, *operands):
     """`out` checked, or a new tensor on `like`'s device."""
     if out is None:
         return like.new_empty(shape, dtype=dtype)
+    begin, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
+    for t in (like,) + operands:   # (of operands with strides: from the first to the last element)
+        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else -1
+        if begin < t.data_ptr() + (last + 1) * t.element_size() and t.data_ptr() < end:
+            raise RockError("%s: out overlaps an operand" % name)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
         raise RockError("%s: out must be %s of %s on %s" % (name, tuple(shape), dtype, like.device))
     if not out.is_contiguous() or out.data_ptr() & 15:
@@ -1056,7 +1061,7 @@ def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, a
                    _scale_vector(name, "token_scale", token_scale, M)]
         if vector:
             tensors.append(_scale_vector(name, "scale", scale, N))
-        res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a)
+        res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a, b)
         if M == 0:
             return res
         lo, hi = (None, None) if clip is None else (float(clip[0]), float(clip[1]))
@@ -1118,7 +1123,7 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
             tensors.append(_scale_vector(name, "token_scale", token_scale, T))
         if vector:
             tensors.append(_scale_vector(name, "scale", scale, E * N))
-        res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x)
+        res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x, w, offsets)
         if T == 0 or N == 0:
             return res
         prog = _token_plan("operation t g m n k transB out_datatype token_scale_vector scale_vector scale perf_config", name, t,
@@ -1141,7 +1146,7 @@ def grouped_gemm_bwd_data(dout, w, offsets, *, transB=False, out=None, stream=No
         raise RockError("%s: f16, bf16 or f32 operands" % name)
     _same_device(name, dout, w=w, offsets=offsets)
     with _on(name, dout.device, stream):
-        res = _result(name, out, (T, K), dout.dtype, dout)
+        res = _result(name, out, (T, K), dout.dtype, dout, w, offsets)
         if T == 0 or K == 0:
             return res
         prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
@@ -1165,7 +1170,7 @@ def grouped_gemm_bwd_weight(x, dout, offsets, *, transB=False, out=None, stream=
         raise RockError("%s: f16, bf16 or f32 operands" % name)
     _same_device(name, x, dout=dout, offsets=offsets)
     with _on(name, x.device, stream):
-        res = _result(name, out, (E, N, K) if transB else (E, K, N), x.dtype, x)
+        res = _result(name, out, (E, N, K) if transB else (E, K, N), x.dtype, x, dout, offsets)
         if res.numel() == 0:
             return res
         if T == 0:

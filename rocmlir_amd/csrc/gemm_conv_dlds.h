@@ -922,7 +922,6 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
       char *wbuf = lds + wave * WBUF;
 #pragma unroll
       for (int i = 0; i < MI; ++i) {
-        const auto rv = row_values(p, m_wave + i * 32 + lrow);
 #pragma unroll
         for (int j = 0; j < NI; ++j) {
 #pragma unroll
@@ -930,7 +929,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
             const int nloc = j * 32 + q * 8 + lgrp * 4;
             Acc4 a4 = {acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                        acc[i][j][4 * q + 3]};
-            const v4i raw = tile_convert4<Tr::INT_ACC, OD>(a4, p, rv, aux, n_wave + nloc);
+            const v4i raw = epilogue_convert4<Tr::INT_ACC, OD>(a4, e, aux, n_wave + nloc, p.N);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               char *dst = wbuf + (nloc + r) * MP + lrow * ES;
@@ -978,7 +977,6 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
     const int rd_row = lane / LPR, rd_cb = (lane % LPR) * 16;
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-      const auto rv = row_values(p, m_wave + i * 32 + lrow);
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
 #pragma unroll
@@ -986,7 +984,7 @@ __device__ __forceinline__ void dl_epilogue(typename MmaTraits<DT>::Acc (&acc)[M
           const int nloc = j * 32 + q * 8 + lgrp * 4;
           Acc4 a4 = {acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                      acc[i][j][4 * q + 3]};
-          v4i raw = tile_convert4<Tr::INT_ACC, OD>(a4, p, rv, aux, n_wave + nloc);
+          v4i raw = epilogue_convert4<Tr::INT_ACC, OD>(a4, e, aux, n_wave + nloc, p.N);
           char *dst = wbuf + lrow * PITCH + nloc * ES;
           if constexpr (ES == 4)
             *(v4i *)dst = raw;

@@ -673,17 +673,6 @@ __device__ __forceinline__ auto make_loader_b(const void *fil, const RockConvPar
   return l;
 }
 
-// What the epilogue of output row m needs beside the parameter block, fetched once per row, and the conversion of
-// four channels of that row.  Nothing for these parameter blocks; a product with a scale for each row (token_gemm.h)
-// overloads both for its own.
-struct NoRowValues {};
-template <typename Params> __device__ __forceinline__ NoRowValues row_values(const Params &, int) { return {}; }
-template <bool INT_ACC, int OD, bool SLOW_CALL = false, bool CHAN = false, typename Acc4, typename Params>
-__device__ __forceinline__ v4i tile_convert4(const Acc4 &acc, const Params &p, NoRowValues, const void *aux, int n0,
-                                             const void *res = nullptr, int64_t res_off = 0, int64_t res_ns = 1) {
-  return epilogue_convert4<INT_ACC, OD, SLOW_CALL, CHAN>(acc, p.epi, aux, n0, p.N, res, res_off, res_ns);
-}
-
 // Epilogue straight from the accumulator layout: the lane owns rows
 // m_lane + 32*i and channels n_lane + 32*j + 8*q + {0..3}.
 template <bool INT_ACC, int OD, int MI, int NI, typename Acc4, bool SLOW_CALL = true, typename AccArr, typename Params>
@@ -698,7 +687,6 @@ __device__ __forceinline__ void direct_epilogue(const AccArr &acc, const Params 
     int64_t row_off, n_stride;
     bool vec_ok;
     out_row_addr(p, g, m, Cptr, row_off, n_stride, vec_ok);
-    const auto rv = row_values(p, m);
 #pragma unroll
     for (int j = 0; j < NI; ++j) {
 #pragma unroll
@@ -709,7 +697,7 @@ __device__ __forceinline__ void direct_epilogue(const AccArr &acc, const Params 
         Acc4 a4 = {acc[i][j][4 * q + 0], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
                    acc[i][j][4 * q + 3]};
         // (the callers that take every epilogue -- SLOW_CALL -- also take the per-channel vectors)
-        v4i raw = tile_convert4<INT_ACC, OD, SLOW_CALL, SLOW_CALL>(a4, p, rv, aux, n, p.epi.residual_op ? res : nullptr,
+        v4i raw = epilogue_convert4<INT_ACC, OD, SLOW_CALL, SLOW_CALL>(a4, p.epi, aux, n, p.N, p.epi.residual_op ? res : nullptr,
                                                  row_off + (int64_t)n * n_stride, n_stride);
         store_packed4(raw, ES, Cptr, row_off + (int64_t)n * n_stride, n_stride, n, p.N, vec_ok);
       }
@@ -718,12 +706,11 @@ __device__ __forceinline__ void direct_epilogue(const AccArr &acc, const Params 
 }
 
 // ---------------------------------------------------------------------------
-// The kernel body: the output tile (g, m0.., n0..) by the calling block.
-// IS_CONV selects the parameter block type.
+// The kernel body.  IS_CONV selects the parameter block type.
 // ---------------------------------------------------------------------------
 template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int LDA, int LDB, typename Params>
-__device__ __forceinline__ void contraction_tile(const void *Aptr, const void *Bptr, void *Cptr, const void *aux,
-                                                 const void *res, const Params &p, int g, int m0, int n0) {
+__device__ __forceinline__ void contraction_body(const void *Aptr, const void *Bptr, void *Cptr,
+                                                 const void *aux, const void *res, const Params &p) {
   using Tr = MmaTraits<DT>;
   using Acc = typename Tr::Acc;
   constexpr int NT = WAVES_M * WAVES_N * 64;
@@ -739,6 +726,10 @@ __device__ __forceinline__ void contraction_tile(const void *Aptr, const void *B
   const int lane = tid & 63, wave = tid >> 6;
   const int wm = wave % WAVES_M, wn = wave / WAVES_M;
   const int lrow = lane & 31, lgrp = lane >> 5;
+
+  int g, tm, tn;
+  decode_block(p.tiles_m, p.tiles_n, p_batch(p), p.group_m, p.xcd_remap, g, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
 
   // ---- loaders
   using GA = TileGeom<DT, BM, NT>;
@@ -800,20 +791,13 @@ __device__ __forceinline__ void contraction_tile(const void *Aptr, const void *B
   Params pg = p;
   const void *aux_g = aux;
   group_channel_pointers(pg, aux_g, g);
+  const RockEpilogue &e = pg.epi;
   using Acc4 = decltype(__builtin_shufflevector(acc[0][0], acc[0][0], 0, 1, 2, 3));
-  dispatch_tile_dtype<Tr::INT_ACC>(pg, [&](auto od_const) __attribute__((always_inline)) {
+  dispatch_out_dtype<Tr::INT_ACC>(e.out_dtype, [&](auto od_const) __attribute__((always_inline)) {
     constexpr int OD = decltype(od_const)::value;
     direct_epilogue<Tr::INT_ACC, OD, MI, NI, Acc4>(acc, pg, g, Cptr, aux_g, res, m0 + wm * WTM + lrow,
                                                   n0 + wn * WTN + lgrp * 4);
   });
-}
-
-template <int DT, int BM, int BN, int WAVES_M, int WAVES_N, int LDA, int LDB, typename Params>
-__device__ __forceinline__ void contraction_body(const void *Aptr, const void *Bptr, void *Cptr,
-                                                 const void *aux, const void *res, const Params &p) {
-  int g, tm, tn;
-  decode_block(p.tiles_m, p.tiles_n, p_batch(p), p.group_m, p.xcd_remap, g, tm, tn);
-  contraction_tile<DT, BM, BN, WAVES_M, WAVES_N, LDA, LDB>(Aptr, Bptr, Cptr, aux, res, p, g, tm * BM, tn * BN);
 }
 
 } // namespace rk

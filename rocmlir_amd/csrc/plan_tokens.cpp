@@ -25,6 +25,13 @@ double tile_time(const TokenTile &t, int64_t tiles) {
   return (double)(tiles / kNumCU) + (left == 0 ? 0.0 : left * 4 <= kNumCU ? 0.4 : left * 2 <= kNumCU ? 0.6 : 1.0);
 }
 
+const TokenTile *requested_tile(const OptMap &o) {
+  for (const TokenTile &t : kTokenTiles)
+    if (requested_tile_is(o, t.bm, t.bn))
+      return &t;
+  return nullptr;
+}
+
 // Kernels for few rows (csrc/token_gemm.h): a block of eight waves per tile, K divided over the waves.
 const TokenTile kSkinnyTiles[] = {{"_16x16_skinny", 16, 16, 1, 8, 0.0}, {"_16x32_skinny", 16, 32, 1, 8, 0.0},
                                   {"_32x16_skinny", 32, 16, 1, 8, 0.0}, {"_32x32_skinny", 32, 32, 1, 8, 0.0}};
@@ -40,7 +47,7 @@ const TokenTile *pick_skinny_tile(int64_t rows, int64_t groups, int64_t cols, bo
   for (const TokenTile &t : kSkinnyTiles)
     if (requested_tile_is(o, t.bm, t.bn))
       return &t;
-  if (o.count("perf_config"))
+  if (requested_tile(o))
     return nullptr;
   const int64_t used = std::min(rows, groups), per_group = ceil_div(rows, used);
   for (int i : {0, 1, 2, 3})
@@ -62,13 +69,6 @@ int64_t row_tiles(int64_t rows, int64_t groups, int64_t bm) {
 int64_t expected_row_tiles(int64_t rows, int64_t groups, int64_t bm) {
   const int64_t used = std::min(rows, groups);
   return used * ceil_div(ceil_div(rows, used), bm);
-}
-
-const TokenTile *requested_tile(const OptMap &o) {
-  for (const TokenTile &t : kTokenTiles)
-    if (requested_tile_is(o, t.bm, t.bn))
-      return &t;
-  return nullptr;
 }
 
 // The tile with the least time for a product of `rows` rows in `groups` groups with `cols` columns.

@@ -32,36 +32,36 @@ struct TokenScaleParams : TokenTileParams {
   const float *token_scale;   // of the tile's group: element m belongs to row m
   const float *channel_scale; // element n to column n; NULL: epi.scale
 };
-struct TokenRowValues {
-  float scale;
-};
-__device__ __forceinline__ TokenRowValues row_values(const TokenScaleParams &p, int m) {
-  return {p.token_scale && m < p.M ? p.token_scale[m] : 1.0f};
+__device__ __forceinline__ float token_scale_of(const TokenScaleParams &p, int m) {
+  return p.token_scale && m < p.M ? p.token_scale[m] : 1.0f;
 }
-// (acc - zero_point) * s[n] * t[m] + bias[n], clamped: every step one f32 operation, narrowed once at the end
-template <bool INT_ACC, int OD, bool SLOW_CALL = false, bool CHAN = false, typename Acc4>
-__device__ __forceinline__ v4i tile_convert4(const Acc4 &acc, const TokenScaleParams &p, TokenRowValues row,
-                                             const void *aux, int n0, const void * = nullptr, int64_t = 0,
-                                             int64_t = 1) {
+// One element: (sum - zero_point) * s[n] * t[m] + bias[n], clamped, every step one f32 operation, narrowed once
+// afterwards.  A NaN stays one: it says that the row's activations held an infinity or a NaN.
+__device__ __forceinline__ float scaled_value(int sum, float zero_point, float s, float t, float b, const RockEpilogue &e) {
+  float v = ((float)sum - zero_point) * s * t;
+  if (e.has_bias)
+    v = v + b;
+  if (e.activation && v == v)
+    v = activation_fast(v, e);
+  return v;
+}
+// four channels of row m, packed in the result's type
+template <int OD>
+__device__ __forceinline__ v4i token_convert4(const v4i &acc, const TokenScaleParams &p, int m, const void *bias, int n0) {
   const RockEpilogue &e = p.epi;
-  float s4[4] = {e.scale, e.scale, e.scale, e.scale}, b4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, v[4];
+  const float t = token_scale_of(p, m);
+  float v[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (n0 + r < p.N) {
-      if (p.channel_scale)
-        s4[r] = p.channel_scale[n0 + r];
-      if (e.has_bias)
-        b4[r] = ((const float *)aux)[n0 + r];
-    }
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    v[r] = ((float)(int)acc[r] - (float)e.zero_point) * s4[r] * row.scale;
-    if (e.has_bias)
-      v[r] = v[r] + b4[r];
-    if (e.activation)
-      v[r] = activation_fast(v[r], e);
+  for (int r = 0; r < 4; ++r) { // (channels behind the last one: any value, they are not stored)
+    const int n = min(n0 + r, p.N - 1);
+    v[r] = scaled_value(acc[r], (float)e.zero_point, p.channel_scale ? p.channel_scale[n] : e.scale, t,
+                        e.has_bias ? ((const float *)bias)[n] : 0.0f, e);
   }
   return epilogue_pack4<OD>(v, e);
+}
+template <int OD>
+__device__ __forceinline__ v4i token_convert4(const v4f &acc, const TokenTileParams &p, int, const void *bias, int n0) {
+  return epilogue_convert4<false, OD>(acc, p.epi, bias, n0, p.N);
 }
 
 // Epilogue of the tiled kernels with these scales.  The raw sums go through the wave's LDS region, 32 rows at a time,
@@ -107,20 +107,14 @@ __device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (
         const int row = r0 + rd_row, m = m_wave + i * 32 + row;
         const v4i lo = *(const v4i *)(wbuf + row * PITCH + rd_col * 4);
         const v4i hi = *(const v4i *)(wbuf + row * PITCH + rd_col * 4 + 16);
-        const float t = row_values(p, m).scale;
+        const float t = token_scale_of(p, m);
         v4i out[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int sum = h ? hi[k] : lo[k];
-            v[k] = ((float)sum - zero_point) * s[4 * h + k] * t;
-            if (e.has_bias)
-              v[k] = v[k] + b[4 * h + k];
-            if (e.activation)
-              v[k] = activation_fast(v[k], e);
-          }
+          for (int k = 0; k < 4; ++k)
+            v[k] = scaled_value(h ? hi[k] : lo[k], zero_point, s[4 * h + k], t, b[4 * h + k], e);
           out[h] = epilogue_pack4<OD>(v, e);
         }
         if (m >= p.M)
@@ -707,11 +701,10 @@ __device__ __forceinline__ void skinny_tile(const void *A, const void *B, void *
   int64_t row_off, n_stride;
   bool vec_ok;
   out_row_addr(p, 0, m, C, row_off, n_stride, vec_ok);
-  const auto rv = row_values(p, m);
   dispatch_tile_dtype<MmaTraits<DT>::INT_ACC>(p, [&](auto od_const) __attribute__((always_inline)) {
     constexpr int OD = decltype(od_const)::value;
-    const v4i raw = tile_convert4<MmaTraits<DT>::INT_ACC, OD>(sum, p, rv, bias, n);
-    store_packed4(raw, OutElemSize<OD>::value, C, row_off + n, n_stride, n, p.N, vec_ok && ((row_off + n) & 3) == 0);
+    const v4i raw = token_convert4<OD>(sum, p, m, bias, n);
+    store_packed4(raw, OutElemSize<OD>::value, C, row_off + n, n_stride, n, p.N, vec_ok);
   });
 }
 

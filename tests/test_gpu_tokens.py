@@ -137,6 +137,13 @@ def test_a_poisoned_token_poisons_its_own_row(rock, gpu):
     bad = torch.zeros(40, dtype=torch.bool)
     bad[[7, 30]] = True
     assert y[bad].isnan().all() and y[~bad].isfinite().all()
+    for kw in (dict(relu=True), dict(clip=(-1.0, 1.0))):      # a clamp leaves a NaN alone, few rows or many
+        for rows in (slice(0, 8), slice(0, 40)):
+            y = rock.gemm(q[rows], w, transB=True, token_scale=s[rows], **kw).cpu()
+            assert y[bad[rows]].isnan().all() and y[~bad[rows]].isfinite().all()
+    off = make_offsets([8, 0, 32]).to(gpu)
+    y = rock.grouped_gemm(q, w.expand(3, 96, 256), off, transB=True, token_scale=s).cpu()
+    assert y[bad].isnan().all() and y[~bad].isfinite().all()
 
 
 # ---- products grouped by expert ---------------------------------------------------------------------------------

@@ -46,6 +46,9 @@ I8 = torch.int8
     (lambda r: r.grouped_gemm_bwd_weight(_t(5, 8), _t(4, 6), OFF3), "of one type"),
     (lambda r: r.grouped_gemm_bwd_weight(_t(5, 8), _t(5, 6), OFF3, out=_t(3, 6, 8)), "out must be"),
     (lambda r: r.grouped_gemm_bwd_weight(_t(5, 8), _t(5, 6), OFF3.float()), "offsets is int32"),
+    (lambda r: (lambda x: r.grouped_gemm(x, _t(1, 8, 8), OFF3[:2], transB=True, out=x))(_t(5, 8)), "overlaps an operand"),
+    (lambda r: (lambda b: r.grouped_gemm(b[:5], _t(1, 8, 8), OFF3[:2], transB=True, out=b[4:9]))(_t(9, 8)), "overlaps an operand"),
+    (lambda r: (lambda b: r.grouped_gemm_bwd_weight(_t(5, 8), b[0, :5], OFF3[:2], out=b[:, :8]))(_t(1, 16, 6)), "overlaps an operand"),
     # tensors that pass every check but do not live on a GPU
     (lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), OFF3, transB=True), "must live on the GPU"),
     (lambda r: r.quantize_tokens(_t(5, 8)), "must live on the GPU"),
