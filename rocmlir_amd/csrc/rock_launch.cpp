@@ -105,8 +105,17 @@ bool check_launch_args(Handle *h, void *const *pointers, int num_pointers) {
   }
   if (h->op == OP_TOKENS)
     need_aux = true; // no bias slot: every pointer is a tensor
+  // a conversion kernel reads and writes the tensors of its own map; the problem's optional ones may be missing
+  auto touched = [&](int i) {
+    if (h->op != OP_RELAYOUT || h->ptr_map.empty())
+      return true;
+    for (const Handle::PtrSrc &m : h->ptr_map)
+      if (m.source == i)
+        return true;
+    return false;
+  };
   for (int i = 0; i < num_pointers; ++i)
-    if (!pointers[i] && (i != aux_index || need_aux)) {
+    if (!pointers[i] && (i != aux_index || need_aux) && touched(i)) {
       set_error("launch: NULL tensor pointer");
       return false;
     }
