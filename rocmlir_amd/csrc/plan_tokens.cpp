@@ -131,8 +131,8 @@ bool parse_token_problem(const OptMap &o, const char *what, bool grouped, TokenP
     return fail("operands are f32, f16, bf16 or i8");
   q.G = int_or(o, "g", 1);
   if (!get_int(o, "m", q.T) || !get_int(o, "n", q.N) || !get_int(o, "k", q.K) || q.G <= 0 || q.T <= 0 || q.N <= 0 ||
-      q.K <= 0 || q.T > INT32_MAX - 512 || q.N > INT32_MAX - 512 || q.K > INT32_MAX - 512 || q.G > (1 << 20))
-    return fail("-m, -n, -k (and -g) must be given, positive and within 31 bits (-g: 20 bits)");
+      q.K <= 0 || q.T > INT32_MAX - 512 || q.N > INT32_MAX - 512 || q.K > INT32_MAX - 512 || q.G > 65536)
+    return fail("-m, -n, -k (and -g) must be given, positive and within 31 bits (-g: at most 65536, every block reads the offsets)");
   q.transB = bool_or(o, "transB", false);
   if (bool_or(o, "transA", false) || bool_or(o, "transC", false))
     return fail("the token rows of operand and result are contiguous (no transA, transC)");

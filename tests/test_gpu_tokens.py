@@ -213,6 +213,57 @@ def test_gradients_against_differences(rock, gpu):
     assert ((f(x, w + v) - f(x, w - v)) * dout).sum() / 2 == (dw.double() * v).sum()
 
 
+TILES = ["16,16", "16,32", "32,16", "32,32", "64,64", "128,128", "256,256"]
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("n,k", [(272, 208), (205, 131)], ids=["chunks", "any"])
+@pytest.mark.parametrize("transB", [True, False], ids=["NK", "KN"])
+@pytest.mark.parametrize("t", FLOATS + ("i8",))
+def test_every_kernel(rock, gpu, t, transB, n, k, tile):
+    """Every tile of every product and gradient, by request: groups that end inside a tile, at its end and one row
+    behind it, an empty one, rows of none.  Exact sums."""
+    sizes, tail = [64, 0, 257, 129, 1, 16], 3
+    g, T, E = generator(n + k), sum(sizes) + tail, len(sizes)
+    kind = torch.int8 if t == "i8" else TORCH[t]
+    x, w, dout = whole(g, -2, 2, T, k).to(kind), whole(g, -2, 2, E, n, k).to(kind), whole(g, -2, 2, T, n).to(kind)
+    wd = (w if transB else w.transpose(1, 2).contiguous()).to(gpu)
+    off, xd, dd = make_offsets(sizes).to(gpu), x.to(gpu), dout.to(gpu)
+    perf, info = "v2:" + tile, {}
+    y = torch.full((T, n), -7.0, dtype=torch.float32, device=gpu)
+    rock.grouped_gemm(xd, wd, off, transB=transB, out_dtype="f32", out=y, perf_config=perf, info=info)
+    if transB:      # (the kernels for few rows take weights stored [N, K] only, those of any alignment have no 256 x 256)
+        assert tile.replace(",", "x") in info["kernel_name"] or (tile == "256,256" and "_any" in info["kernel_name"])
+    for e, a, b in spans(sizes):
+        assert torch.equal(y[a:b].cpu(), (x[a:b].double() @ w[e].double().t()).float()), (info, e)
+    assert (y[sum(sizes):] == -7).all()
+    if t == "i8":
+        return
+    dx = rock.grouped_gemm_bwd_data(dd, wd, off, transB=transB, perf_config=perf)
+    dw = rock.grouped_gemm_bwd_weight(xd, dd, off, transB=transB, perf_config=perf)
+    for e, a, b in spans(sizes):
+        assert torch.equal(dx[a:b].cpu(), (dout[a:b].double() @ w[e].double()).to(kind)), e
+        want = dout[a:b].double().t() @ x[a:b].double()
+        assert torch.equal(dw[e].cpu(), (want if transB else want.t()).to(kind)), e
+
+
+@pytest.mark.parametrize("t,n,k", [("bf16", 2056, 72), ("f32", 1100, 40)])
+def test_tiles_in_whole_rounds_and_parts(rock, gpu, t, n, k):
+    """More 256 x 256 tiles than compute units in the product and both gradients, so that whole tiles, halves and
+    quarters run in one launch."""
+    sizes = [300, 1, 0, 2000, 513, 256, 40, 700]
+    g, T, E = generator(n), sum(sizes), len(sizes)
+    x, w, dout = (whole(g, -1, 1, *s).to(TORCH[t]).to(gpu) for s in ((T, k), (E, n, k), (T, n)))
+    off = make_offsets(sizes).to(gpu)
+    kw = dict(transB=True, perf_config="v2:256,256")
+    y, dw = rock.grouped_gemm(x, w, off, **kw), rock.grouped_gemm_bwd_weight(x, dout, off, **kw)
+    wide = rock.grouped_gemm_bwd_data(x, w.transpose(1, 2).contiguous(), off, **kw)     # as dout [T, k] of weights [E, k, n]
+    for e, a, b in spans(sizes):
+        want = (x[a:b].cpu().double() @ w[e].cpu().double().t()).to(TORCH[t])
+        assert torch.equal(y[a:b].cpu(), want) and torch.equal(wide[a:b].cpu(), want), e
+        assert torch.equal(dw[e].cpu(), (dout[a:b].cpu().double().t() @ x[a:b].cpu().double()).to(TORCH[t])), e
+
+
 @pytest.mark.parametrize("out", FLOATS)
 @pytest.mark.parametrize("transB", [True, False], ids=["NK", "KN"])
 @pytest.mark.parametrize("case", CASES, ids=_ids)

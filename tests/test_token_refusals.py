@@ -66,6 +66,7 @@ def test_entry_points_refuse(rock, call, text):
     ("-operation grouped_gemm -t fp8 -g 2 -m 4 -n 8 -k 16", "operands are"),
     ("-operation grouped_gemm -t f16 -g 0 -m 4 -n 8 -k 16", "positive"),
     ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8", "positive"),
+    ("-operation grouped_gemm -t f16 -g 65537 -m 4 -n 8 -k 16", "at most 65536"),
     ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8 -k 16 -transA true", "no transA"),
     ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8 -k 16 -bias true", "no bias"),
     ("-operation grouped_gemm -t f16 -g 2 -m 4 -n 8 -k 16 -token_scale_vector true", "scales go with int8"),
