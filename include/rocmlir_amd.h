@@ -77,6 +77,25 @@ typedef void *MiirHandle;
  * for i8, over tensors contiguous along the head dimension: transK, no other
  * transpose); f32, larger head dimensions and "-fused false" run as three
  * kernels over a score workspace.
+ * Operators over the token rows of a language model, without a counterpart in
+ * the reference, one kernel each, no workspace:
+ *   quantize_tokens (t f32|f16|bf16, m rows, k columns; pointers x [m,k],
+ *     q int8 [m,k], scale f32 [m]): scale = max |x| / 127 and
+ *     q = roundeven(127 x / max |x|) row by row; a row of zeros has scale 0, a
+ *     row with an infinity or a NaN scale NaN and q = 0;
+ *   gemm with "token_scale_vector true" (t i8, g 1, transB, out_datatype f16
+ *     (default)|bf16|f32; pointers A, B, C, bias slot, token scales f32 [m],
+ *     [channel scales f32 [n] with "scale_vector true"]):
+ *     C = (A B - zero_point) * scale[n] * token[m] + bias, then relu or clip;
+ *   grouped_gemm (t f32|f16|bf16|i8, g groups, m rows, n, k, transB): row m of
+ *     x [m,k] times the weights [g,k,n] ([g,n,k] with transB) of the group whose
+ *     range [offsets[e], offsets[e+1]) holds it; pointers x, weights, result,
+ *     offsets int32 [g+1] in device memory, [token scales [m]], [channel scales
+ *     [g,n]].  Rows of no group are not written; an offset that steps back or
+ *     lies outside [0, m] is read as the furthest one before it;
+ *   grouped_gemm_bwd_data, grouped_gemm_bwd_weight: its gradients, with its keys
+ *     and pointer order, the gradient written in its own slot (weights of a
+ *     group without rows: zeros).
  * Epilogue keys (all optional): scale, zero_point, quant_scale,
  * out_zero_point, bias, relu; and the element-wise operations MIGraphX fuses
  * behind a contraction (MIGraphXToTosa.cpp:1009-1016, 1089-1100, 1283-1295):
