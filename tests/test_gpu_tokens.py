@@ -27,6 +27,11 @@ def whole(g, lo, hi, *shape):
     return torch.randint(lo, hi + 1, shape, generator=g)
 
 
+def _device_only(gpu):
+    if gpu.type != "cuda":     # (the CPU build of the kernels in place of the device: kernel_host/as_device.py)
+        pytest.skip("streams, graphs and gigabytes are not the model's business")
+
+
 def make_offsets(sizes):
     return torch.from_numpy(np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32))
 
@@ -333,6 +338,7 @@ def test_no_rows_at_all(rock, gpu):
 
 def test_rows_behind_two_gibibytes(rock, gpu):
     """Rows whose byte positions pass 2^31 and 2^32, in the operands of the product and of both gradients."""
+    _device_only(gpu)
     n, k, T = 2048, 32, 1_100_000                       # dout: 4.5 GB
     sizes = [520_000, 530_000, 49_990]                  # groups start at 2.1 GB and 4.3 GB of dout
     off = make_offsets(sizes).to(gpu)
@@ -398,6 +404,7 @@ def test_int8_experts_from_tokens_to_tokens(rock, gpu):
 def test_a_training_step_replayed_from_a_graph(rock, gpu):
     """Forward and both gradients of a grouped product, and a quantised product, captured once and replayed on new
     inputs, offsets included, with eager work between the replays: equal to the eager calls bit for bit."""
+    _device_only(gpu)
     E, T, n, k = 6, 200, 136, 96
     g = generator(31)
     x, dout = torch.zeros((T, k), dtype=torch.bfloat16, device=gpu), torch.zeros((T, n), dtype=torch.bfloat16, device=gpu)
@@ -434,6 +441,7 @@ def test_a_training_step_replayed_from_a_graph(rock, gpu):
 def test_streams_and_threads(rock, gpu):
     """The same problem from two threads on streams of their own, operands made on those streams; and a stream passed
     by argument, as an object and as a raw handle."""
+    _device_only(gpu)
     g = generator(41)
     sizes, n, k = [50, 3, 90], 200, 160
     off = make_offsets(sizes).to(gpu)
