@@ -129,6 +129,8 @@ def token_kernels(type_code):
         if t != "i8":
             out.append(("rock_token_gemm_bwd_weight_%s%s" % (t, tile),
                         "RK_TOKEN_WEIGHT_DL(%s, %s, %d, %d)" % ((tile, dims) + weight[4 if t == "f32" else 2])))
+    if t != "i8":
+        out.append(("rock_token_gemm_bwd_weight_%s_64x64_split" % t, "RK_TOKEN_WEIGHT_SPLIT(_64x64_split)"))
     for tile in ("_128x128", "_64x64"):   # rows of any alignment
         dims = "%d, %d, %d, %d" % TILES[tile]
         for suffix, b_cols in (("_any", "false"), ("_any_nn", "true")):

@@ -313,6 +313,17 @@ Handle *make_grouped_gemm(const OptMap &o) {
       threads = t->waves_m * t->waves_n * 64;
       h->kernel_name = name + t->suffix;
       h->perf_config = token_perf_string(bm, bn, t->waves_m, es);
+      // the reduction over the waves of a block: where the 64 x 64 tiles leave no compute unit two of them and every
+      // share has two K-steps (bf16, us with / without: one result 512 x 512 of 4000 rows 23 / 34, 256 x 256 of 16384 75 /
+      // 126, four 512 x 512 of 1000 rows each 11 / 13, of 250 6.6 / 5.2); splitK, the seventh field of a perf_config,
+      // asks for it or declines it
+      const int64_t tiles = q.G * ceil_div(M, 64) * ceil_div(N, 64), depth = ceil_div(q.T, std::min(q.T, q.G));
+      const bool asked = o.count("perf_config") && bm == 64 && requested_tile(o);
+      if (bm == 64 && (asked ? perf_field(o, 6, 1) == 4 : tiles <= kNumCU && depth * es >= 8 * 128)) {
+        threads = 1024;
+        h->kernel_name = name + "_64x64_split";
+        h->perf_config = with_block_splits(h->perf_config, 4);
+      }
     } else {
       const TokenTile *t = pick_any_tile(q.G * ceil_div(M, 128) * ceil_div(N, 128), o);
       bm = t->bm; bn = t->bn;

@@ -252,6 +252,21 @@ def test_every_kernel(rock, gpu, t, transB, n, k, tile):
         assert torch.equal(dw[e].cpu(), (want if transB else want.t()).to(kind)), e
 
 
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("sizes", [[3000, 0, 33, 1], [64], [257, 512]], ids=str)
+def test_weight_gradient_split_over_the_waves(rock, gpu, t, sizes):
+    case = (sizes, 2, 136, 72)
+    for integers in (True, False):
+        g, T, E, x, w, dout, off = grouped_operands(case, t, True, integers, 17)
+        info = {}
+        dw = rock.grouped_gemm_bwd_weight(x.to(gpu), dout.to(gpu), off.to(gpu), transB=True, info=info,
+                                          perf_config="v2:64,64,8,32,16,8,4,1,1")
+        assert info["kernel_name"].endswith("_64x64_split")
+        for e, a, b in spans(sizes):
+            x64, d64 = x[a:b].double(), dout[a:b].double()
+            check_sum(dw[e], d64.t() @ x64, d64.abs().t() @ x64.abs(), b - a, e)
+
+
 @pytest.mark.parametrize("t,n,k", [("bf16", 2056, 72), ("f32", 1100, 40)])
 def test_tiles_in_whole_rounds_and_parts(rock, gpu, t, n, k):
     """More 256 x 256 tiles than compute units in the product and both gradients, so that whole tiles, halves and

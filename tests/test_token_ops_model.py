@@ -295,6 +295,25 @@ def test_grouped_product_every_kernel_for_few_rows(model, rock, tile, t, n, k):
     assert (res[sum(sizes):].view(np.uint8) == 0xEE).all()
 
 
+@pytest.mark.parametrize("t", ["f16", "f32"])
+@pytest.mark.parametrize("transB", [True, False])
+@pytest.mark.parametrize("sizes", [[700, 0, 33, 1], [64], [257, 512]])
+def test_weight_gradient_split_over_the_waves(model, rock, loads, t, transB, sizes):
+    """Shares with several K-steps, with one, with none; groups without rows."""
+    tail, n, k = 2, 136, 72
+    rng, T, E, offsets, x, w = _problem(sizes, tail, n, k, t, transB)
+    dout = rng.integers(-3, 4, (T, n)).astype(_NUMPY[t])
+    dout[sum(sizes):] = np.nan
+    x[sum(sizes):] = np.nan
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_weight", t, T, E, n, k, transB, "-perf_config v2:64,64,8,32,16,8,4,1,1"),
+                                    {0: x, 2: dout, 3: offsets})
+    assert not problems and names[0].endswith("_64x64_split"), (names, problems)
+    dw = got[1][:w.nbytes].view(w.dtype).reshape(w.shape)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        d64, x64 = dout[a:b].astype(np.float64), x[a:b].astype(np.float64)
+        assert np.array_equal(dw[e].astype(np.float64), (d64.T @ x64 if transB else x64.T @ d64).astype(_NUMPY[t])), e
+
+
 @pytest.mark.parametrize("offsets", [[0, 5, 3, 9], [-4, 2, 100, 7], [4, 4, 4, 2], [9, 0, 0, 0], [2147483647] * 4, [-2147483648, 1, 1, 12]])
 def test_offsets_that_are_no_offsets_stay_inside_the_tensors(model, rock, offsets):
     """Boundaries that step back or lie outside are read as the furthest one before them: nothing outside the tensors
