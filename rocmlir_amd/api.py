@@ -326,17 +326,16 @@ class RockKernel:
                             % (self.kernel_name, rc, last_error()))
 
     def launch_checked(self, args):
-        """launch() on torch's current stream for a caller that has checked the tensors against the problem's sizes
-        and made their device the current one: a call costs the host a third of launch()."""
+        """launch() on torch's current stream for a caller that has checked the tensors against the problem's sizes,
+        that they are on one device and that this device is the current one: a call costs the host a third of
+        launch()."""
         if torch is None:
             _load_torch()
-        arr = self._pointers()
-        for i, a in enumerate(args):
-            if a is not None:
-                if not a.is_cuda:
-                    raise RockError("tensor arguments must live on the GPU")
-                arr[i] = a.data_ptr()
-        rc = _lib.rockamdLaunch(self._h, arr, len(args), torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
+        if not args[0].is_cuda:
+            raise RockError("tensor arguments must live on the GPU")
+        arr = self._pointers(*[None if a is None else a.data_ptr() for a in args])
+        rc = _lib.rockamdLaunch(self._h, arr, self.caller_pointers,
+                                torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()))
         if rc != 0:
             raise RockError("launch of %s failed (hip error %d): %s" % (self.kernel_name, rc, last_error()))
 
@@ -565,13 +564,13 @@ def gemm(a, b, *, transA=False, transB=False, transC=False, out_dtype=None,
     (sum - zero_point) * scale[n] * token_scale[m] (+ bias, then relu or clip)
     in `out_dtype` f16 (the default), bf16 or f32.  K up to 131071; no transA,
     transC, residual, requantisation or accumulation beside it."""
-    import torch
     if token_scale is not None:
         if transA or transC or accumulate or residual is not None or quant_scale is not None or _is_tensor(zero_point) \
                 or _is_tensor(out_zero_point) or out_zero_point:
             raise RockError("gemm: token_scale takes scale, a scalar zero_point, bias, relu and clip only")
         return _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, activation, clip, out,
                                   perf_config, stream, info, token_scale)
+    import torch
     if accumulate and (out is None or residual is not None):
         raise RockError("gemm: accumulate=True adds into `out` and takes no residual")
     a3 = a if a.dim() == 3 else a.unsqueeze(0)
@@ -955,21 +954,24 @@ def _dense(t):
     return t.clone() if t.data_ptr() & 15 else t
 
 
-def _same_device(name, first, **others):
-    for what, t in others.items():
-        if t is not None and t.device != first.device:
-            raise RockError("%s: %s is on %s, the first operand on %s" % (name, what, t.device, first.device))
+def _same_device(name, first, *others):
+    index = first.get_device()      # (-1: the host's memory)
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise RockError("%s: a tensor is on %s, the first operand on %s" % (name, t.device, first.device))
 
 
-_here = contextlib.nullcontext()
+def _elsewhere(device, stream):
+    """The call is for another stream or device than the current ones."""
+    return stream is not None or (device.type == "cuda" and device.index != torch._C._cuda_getDevice())
 
 
 def _on(name, device, stream):
     """A context that makes the operands' device the current one and `stream` (default: the device's current stream)
     torch's current stream, so that copies and results made on the way are ordered with the kernels."""
-    if device.type != "cuda" or (stream is None and device.index == torch._C._cuda_getDevice()):
-        return _here
     stack = contextlib.ExitStack()
+    if device.type != "cuda":
+        return stack
     stack.enter_context(torch.cuda.device(device))
     if stream is not None:
         if not isinstance(stream, torch.cuda.Stream):
@@ -985,10 +987,12 @@ def _result(name, out, shape, dtype, like, *operands):
     """`out` checked, or a new tensor on `like`'s device."""
     if out is None:
         return like.new_empty(shape, dtype=dtype)
-    begin, end = out.data_ptr(), out.data_ptr() + out.numel() * out.element_size()
-    for t in (like,) + operands:   # (of operands with strides: from the first to the last element)
-        last = sum((n - 1) * st for n, st in zip(t.shape, t.stride())) if t.numel() else -1
-        if begin < t.data_ptr() + (last + 1) * t.element_size() and t.data_ptr() < end:
+    begin, end = out.data_ptr(), out.data_ptr() + out.nbytes
+    for t in (like,) + operands:
+        span = t.nbytes   # with strides: from the first to the last element
+        if not t.is_contiguous() and span:
+            span = (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
+        if begin < t.data_ptr() + span and t.data_ptr() < end:
             raise RockError("%s: out overlaps an operand" % name)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
         raise RockError("%s: out must be %s of %s on %s" % (name, tuple(shape), dtype, like.device))
@@ -1003,8 +1007,7 @@ def _launch_tokens(prog, info, *tensors):
         info["kernel_name"] = prog.kernel_name
         info["perf_config"] = prog.perf_config
     with prog.lock:
-        for k in prog.kernels:
-            k.launch_checked(tensors)
+        prog.kernels[0].launch_checked(tensors)   # (these problems have one kernel)
 
 
 def _scale_vector(name, what, t, count):
@@ -1025,13 +1028,15 @@ def quantize_tokens(x, *, out=None, scale_out=None, stream=None, info=None):
     shape = x.shape
     if not shape or x.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise RockError("quantize_tokens: x is [..., K] of f16, bf16 or f32")
-    with _on(name, x.device, stream):
-        q = _result(name, out, shape, torch.int8, x)
-        s = _result(name, scale_out, shape[:-1], torch.float32, x)
-        count, cols = x.numel(), shape[-1]
-        if count == 0:
-            return q, s.zero_()   # rows without elements: their largest magnitude is 0
-        _launch_tokens(_token_plan("operation t m k", name, _dtype_name(x.dtype), count // cols, cols), info, _dense(x), q, s)
+    if _elsewhere(x.device, stream):
+        with _on(name, x.device, stream):
+            return quantize_tokens(x, out=out, scale_out=scale_out, info=info)
+    q = _result(name, out, shape, torch.int8, x)
+    s = _result(name, scale_out, shape[:-1], torch.float32, x)
+    count, cols = x.numel(), shape[-1]
+    if count == 0:
+        return q, s.zero_()   # rows without elements: their largest magnitude is 0
+    _launch_tokens(_token_plan("operation t m k", name, _dtype_name(x.dtype), count // cols, cols), info, _dense(x), q, s)
     return q, s
 
 
@@ -1055,22 +1060,25 @@ def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, a
     if out_dtype not in ("f16", "bf16", "f32"):
         raise RockError("%s: out_dtype f16, bf16 or f32" % name)
     vector = _is_tensor(scale)
-    _same_device(name, a, b=b, token_scale=token_scale, scale=scale if vector else None, bias=bias)
-    with _on(name, a.device, stream):
-        tensors = [_dense(a), _dense(b), None, None if bias is None else _scale_vector(name, "bias", bias, N),
-                   _scale_vector(name, "token_scale", token_scale, M)]
-        if vector:
-            tensors.append(_scale_vector(name, "scale", scale, N))
-        res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a, b)
-        if M == 0:
-            return res
-        lo, hi = (None, None) if clip is None else (float(clip[0]), float(clip[1]))
-        prog = _token_plan("operation t token_scale_vector m n k transB out_datatype scale_vector scale zero_point bias "
-                           "activation clip_min clip_max perf_config", "gemm", "i8", True, M, N, K, bool(transB), out_dtype,
-                           vector, None if vector or scale is None else float(scale), int(zero_point) or None,
-                           bias is not None, "clip" if clip is not None else "relu" if relu else activation, lo, hi,
-                           perf_config)
-        _launch_tokens(prog, info, *tensors)
+    _same_device(name, a, b, token_scale, scale if vector else None, bias)
+    if _elsewhere(a.device, stream):
+        with _on(name, a.device, stream):
+            return _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, activation, clip, out,
+                                      perf_config, None, info, token_scale)
+    tensors = [_dense(a), _dense(b), None, None if bias is None else _scale_vector(name, "bias", bias, N),
+               _scale_vector(name, "token_scale", token_scale, M)]
+    if vector:
+        tensors.append(_scale_vector(name, "scale", scale, N))
+    res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a, b)
+    if M == 0:
+        return res
+    lo, hi = (None, None) if clip is None else (float(clip[0]), float(clip[1]))
+    prog = _token_plan("operation t token_scale_vector m n k transB out_datatype scale_vector scale zero_point bias "
+                       "activation clip_min clip_max perf_config", "gemm", "i8", True, M, N, K, bool(transB), out_dtype,
+                       vector, None if vector or scale is None else float(scale), int(zero_point) or None,
+                       bias is not None, "clip" if clip is not None else "relu" if relu else activation, lo, hi,
+                       perf_config)
+    _launch_tokens(prog, info, *tensors)
     return res
 
 
@@ -1116,20 +1124,23 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
     if out_dtype not in ("f16", "bf16", "f32"):
         raise RockError("%s: out_dtype f16, bf16 or f32" % name)
     vector = _is_tensor(scale)
-    _same_device(name, x, w=w, offsets=offsets, token_scale=token_scale, scale=scale if vector else None)
-    with _on(name, x.device, stream):
-        tensors = [_dense(x), _dense(w), None, _dense(offsets)]
-        if token_scale is not None:
-            tensors.append(_scale_vector(name, "token_scale", token_scale, T))
-        if vector:
-            tensors.append(_scale_vector(name, "scale", scale, E * N))
-        res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x, w, offsets)
-        if T == 0 or N == 0:
-            return res
-        prog = _token_plan("operation t g m n k transB out_datatype token_scale_vector scale_vector scale perf_config", name, t,
-                           E, T, N, K, bool(transB), out_dtype, token_scale is not None, vector,
-                           None if vector or scale is None else float(scale), perf_config)
-        _launch_tokens(prog, info, *tensors)
+    _same_device(name, x, w, offsets, token_scale, scale if vector else None)
+    if _elsewhere(x.device, stream):
+        with _on(name, x.device, stream):
+            return grouped_gemm(x, w, offsets, transB=transB, out_dtype=out_dtype, token_scale=token_scale, scale=scale,
+                                out=out, perf_config=perf_config, info=info)
+    tensors = [_dense(x), _dense(w), None, _dense(offsets)]
+    if token_scale is not None:
+        tensors.append(_scale_vector(name, "token_scale", token_scale, T))
+    if vector:
+        tensors.append(_scale_vector(name, "scale", scale, E * N))
+    res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x, w, offsets)
+    if T == 0 or N == 0:
+        return res
+    prog = _token_plan("operation t g m n k transB out_datatype token_scale_vector scale_vector scale perf_config", name, t,
+                       E, T, N, K, bool(transB), out_dtype, token_scale is not None, vector,
+                       None if vector or scale is None else float(scale), perf_config)
+    _launch_tokens(prog, info, *tensors)
     return res
 
 
@@ -1144,13 +1155,15 @@ def grouped_gemm_bwd_data(dout, w, offsets, *, transB=False, out=None, stream=No
     t = _dtype_name(dout.dtype)
     if t not in ("f32", "f16", "bf16"):
         raise RockError("%s: f16, bf16 or f32 operands" % name)
-    _same_device(name, dout, w=w, offsets=offsets)
-    with _on(name, dout.device, stream):
-        res = _result(name, out, (T, K), dout.dtype, dout, w, offsets)
-        if T == 0 or K == 0:
-            return res
-        prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
-        _launch_tokens(prog, info, res, _dense(w), _dense(dout), _dense(offsets))
+    _same_device(name, dout, w, offsets)
+    if _elsewhere(dout.device, stream):
+        with _on(name, dout.device, stream):
+            return grouped_gemm_bwd_data(dout, w, offsets, transB=transB, out=out, perf_config=perf_config, info=info)
+    res = _result(name, out, (T, K), dout.dtype, dout, w, offsets)
+    if T == 0 or K == 0:
+        return res
+    prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
+    _launch_tokens(prog, info, res, _dense(w), _dense(dout), _dense(offsets))
     return res
 
 
@@ -1168,13 +1181,15 @@ def grouped_gemm_bwd_weight(x, dout, offsets, *, transB=False, out=None, stream=
     t = _dtype_name(x.dtype)
     if t not in ("f32", "f16", "bf16"):
         raise RockError("%s: f16, bf16 or f32 operands" % name)
-    _same_device(name, x, dout=dout, offsets=offsets)
-    with _on(name, x.device, stream):
-        res = _result(name, out, (E, N, K) if transB else (E, K, N), x.dtype, x, dout, offsets)
-        if res.numel() == 0:
-            return res
-        if T == 0:
-            return res.zero_()
-        prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
-        _launch_tokens(prog, info, _dense(x), res, _dense(dout), _dense(offsets))
+    _same_device(name, x, dout, offsets)
+    if _elsewhere(x.device, stream):
+        with _on(name, x.device, stream):
+            return grouped_gemm_bwd_weight(x, dout, offsets, transB=transB, out=out, perf_config=perf_config, info=info)
+    res = _result(name, out, (E, N, K) if transB else (E, K, N), x.dtype, x, dout, offsets)
+    if res.numel() == 0:
+        return res
+    if T == 0:
+        return res.zero_()
+    prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
+    _launch_tokens(prog, info, _dense(x), res, _dense(dout), _dense(offsets))
     return res
