@@ -397,7 +397,10 @@ Handle *make_quantize_tokens(const OptMap &o) {
     return nullptr;
   }
   h->num_pointers = 3;
-  h->problem_key = "quantize_tokens";
+  std::ostringstream key;
+  key << h->arch << '\t' << int_or(o, "num_cu", kNumCU) << "\t-operation quantize_tokens -t " << dtype_name(t) << " -m " << rows
+      << " -k " << cols;
+  h->problem_key = key.str();
   h->args = {{t, {rows, cols}}, {ROCK_I8, {rows, cols}}, {ROCK_F32, {rows}}};
   return h;
 }

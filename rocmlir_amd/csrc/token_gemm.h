@@ -149,16 +149,19 @@ struct GroupScan {
 template <int BM>
 __device__ __forceinline__ void scan_groups(const int32_t *offsets, int G, int M, int base, int lane, GroupScan &carry,
                                             int &start, int &end, int &tiles_end) {
-  const int e = base + lane;
-  end = e < G ? min(max(offsets[e + 1], 0), M) : 0;
-  end = max(end, carry.end);
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int before = lane_value(end, lane >= d ? lane - d : lane);
-    end = max(end, before);
-  }
+  end = min(max(offsets[min(base + lane + 1, G)], 0), M); // (lanes behind the last group: its end, no tiles)
   start = lane_value(end, lane > 0 ? lane - 1 : 0);
   start = lane > 0 ? start : carry.end;
+  if (__builtin_amdgcn_ballot_w64(end < start)) { // some boundary steps back: the running maximum
+    end = max(end, carry.end);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int before = lane_value(end, lane >= d ? lane - d : lane);
+      end = max(end, before);
+    }
+    start = lane_value(end, lane > 0 ? lane - 1 : 0);
+    start = lane > 0 ? start : carry.end;
+  }
   tiles_end = (end - start + BM - 1) / BM;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
