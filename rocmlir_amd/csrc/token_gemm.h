@@ -802,6 +802,26 @@ __device__ __forceinline__ auto make_dl_b(const void *B, const TokenWeightTile<D
   return l;
 }
 
+// Group g's rows among M, as scan_groups reads the boundaries: from the furthest one up to the group's own, so that the
+// gradient sums exactly the rows that the product gave to the group.  Uniform over the block.
+__device__ __forceinline__ void group_rows(const int32_t *offsets, int g, int M, int &row0, int &rows) {
+  const int lane = threadIdx.x & 63, own = offsets[g];
+  int top = 0;
+  for (int base = 0; base <= g; base += 64)
+    top = max(top, offsets[min(base + lane, g)]);
+  if (__builtin_amdgcn_ballot_w64(top > own)) { // some boundary before it lies further on (or this one below 0)
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int other = lane_value(top, lane ^ d);
+      top = max(top, other);
+    }
+  } else {
+    top = own;
+  }
+  row0 = __builtin_amdgcn_readfirstlane(min(top, M));
+  rows = __builtin_amdgcn_readfirstlane(min(max(offsets[g + 1], row0), M)) - row0;
+}
+
 // Group g's rows as the reduction: operands and result moved to the group, gemm.K its number of rows
 template <int DT, typename F>
 __device__ __forceinline__ void with_weight_group(const void *A, const void *B, void *C, const int32_t *offsets,
@@ -809,9 +829,10 @@ __device__ __forceinline__ void with_weight_group(const void *A, const void *B, 
   constexpr int ES = MmaTraits<DT>::ES;
   TokenWeightTile<DT> q;
   static_cast<RockGemmParams &>(q) = wp.gemm;
-  const int lo = min(max(offsets[g], 0), q.K), hi = min(max(offsets[g + 1], lo), q.K);
-  q.K = __builtin_amdgcn_readfirstlane(hi - lo);
-  const int64_t row0 = __builtin_amdgcn_readfirstlane(lo);
+  int first, rows;
+  group_rows(offsets, g, q.K, first, rows);
+  q.K = rows;
+  const int64_t row0 = first;
   f((const char *)A + row0 * q.a_ks * ES, (const char *)B + row0 * q.b_ks * ES,
     (char *)C + (int64_t)g * q.c_gs * token_out_size(q.epi.out_dtype), q);
 }

@@ -489,3 +489,28 @@ def test_streams_and_threads(rock, gpu):
         y = rock.grouped_gemm(xs[0], w, off, transB=True, stream=given)
         s.synchronize()
         assert torch.equal(y, want[0])
+
+
+@pytest.mark.parametrize("offsets", [[0, 5, 3, 9], [-4, 2, 100, 7], [9, 0, 0, 0], [2147483647] * 4, [-2147483648, 1, 1, 12],
+                                     [0, 40, 7] + [8] * 80 + [60, 2, 90] + [0] * 70 + [130, 5]], ids=lambda o: "-".join(map(str, o[:4])))
+@pytest.mark.parametrize("n,k", [(24, 32), (21, 33)], ids=["chunks", "any"])
+@pytest.mark.parametrize("t", FLOATS)
+def test_gradients_on_offsets_out_of_order_or_range(rock, gpu, t, n, k, offsets):
+    """The gradients read the boundaries as the product does (every address checked on the CPU build of the kernels first,
+    tests/test_token_ops_model.py): no row counts in two groups, rows of none are left as they were."""
+    T, E = 131, len(offsets) - 1
+    g = generator(2)
+    x, w, dout = (whole(g, -2, 2, *s).to(TORCH[t]) for s in ((T, k), (E, n, k), (T, n)))
+    off = torch.tensor(offsets, dtype=torch.int32, device=gpu)
+    at = np.maximum.accumulate(np.clip(np.asarray(offsets, np.int64), 0, T))
+    for perf in (None, "v2:64,64,8,32,16,8,4,1,1", "v2:128,128", "v2:256,256"):
+        dw = rock.grouped_gemm_bwd_weight(x.to(gpu), dout.to(gpu), off, transB=True, perf_config=perf).cpu()
+        for e in range(E):
+            a, b = at[e], at[e + 1]
+            assert torch.equal(dw[e], (dout[a:b].double().t() @ x[a:b].double()).to(TORCH[t])), (perf, e)
+    dx = torch.full((T, k), -7.0, dtype=TORCH[t], device=gpu)
+    rock.grouped_gemm_bwd_data(dout.to(gpu), w.to(gpu), off, transB=True, out=dx)
+    want = torch.full((T, k), -7.0, dtype=TORCH[t])
+    for e in range(E):
+        want[at[e]:at[e + 1]] = (dout[at[e]:at[e + 1]].double() @ w[e].double()).to(TORCH[t])
+    assert torch.equal(dx.cpu(), want)

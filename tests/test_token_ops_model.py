@@ -343,3 +343,34 @@ def test_offsets_that_are_no_offsets_stay_inside_the_tensors(model, rock, offset
     for op, inputs in (("grouped_gemm_bwd_data", {1: w, 2: dout, 3: off}), ("grouped_gemm_bwd_weight", {0: x, 2: dout, 3: off})):
         names, problems, _ = run_plan(model, rock, _opts(op, "f16", T, 3, n, k, True), inputs)
         assert not problems, (names, problems)
+
+
+# boundaries that step back right away, out of the rows, and far behind the furthest one (another lane group's)
+STEPPING_BACK = [[0, 5, 3, 9], [-4, 2, 100, 7], [9, 0, 0, 0], [2147483647] * 4, [-2147483648, 1, 1, 12], [3, 2, 1, 0, 200, 150, 131],
+                 [0, 40, 7] + [8] * 80 + [60, 2, 90] + [0] * 70 + [130, 5]]
+
+
+@pytest.mark.parametrize("offsets", STEPPING_BACK, ids=lambda o: "-".join(map(str, o[:7])))
+@pytest.mark.parametrize("n,k,perf", [(24, 32, ""), (24, 32, "v2:64,64,8,32,16,8,4,1,1"), (24, 32, "v2:128,128"), (24, 32, "v2:256,256"),
+                                      (21, 33, "v2:64,64"), (21, 33, "v2:128,128")],
+                         ids=["chosen", "split", "128", "256", "any64", "any128"])
+def test_gradients_on_offsets_that_step_back(model, rock, offsets, n, k, perf):
+    """Both gradients read the boundaries as the product does: a row counts in one group's gradient at most."""
+    T, E = 131, len(offsets) - 1
+    rng = np.random.default_rng(7)
+    x, w = rng.integers(-3, 4, (T, k)).astype(np.float16), rng.integers(-3, 4, (E, n, k)).astype(np.float16)
+    dout = rng.integers(-3, 4, (T, n)).astype(np.float16)
+    off = np.asarray(offsets, np.int64).astype(np.int32)
+    extra = "-perf_config " + perf if perf else ""
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_weight", "f16", T, E, n, k, True, extra), {0: x, 2: dout, 3: off})
+    assert not problems, (names, problems)
+    dw = got[1][:w.nbytes].view(w.dtype).reshape(w.shape)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        assert np.array_equal(dw[e].astype(np.float64), dout[a:b].astype(np.float64).T @ x[a:b].astype(np.float64)), (names, e)
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_data", "f16", T, E, n, k, True), {1: w, 2: dout, 3: off})
+    assert not problems, (names, problems)
+    dx, owned = got[0][:x.nbytes].view(x.dtype).reshape(T, k), np.zeros(T, bool)
+    for e, (a, b) in enumerate(bounds(offsets, T)):
+        assert np.array_equal(dx[a:b].astype(np.float64), dout[a:b].astype(np.float64) @ w[e].astype(np.float64)), (names, e)
+        owned[a:b] = True
+    assert (dx[~owned].view(np.uint8) == 0xEE).all()
