@@ -975,7 +975,9 @@ def _on(name, device, stream):
     stack.enter_context(torch.cuda.device(device))
     if stream is not None:
         if not isinstance(stream, torch.cuda.Stream):
-            stream = torch.cuda.ExternalStream(int(getattr(stream, "cuda_stream", stream)), device=device)
+            handle = int(getattr(stream, "cuda_stream", stream))
+            # (handle 0 is the default stream; ExternalStream(0) would be one of torch's own, ordered with nothing)
+            stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
         if stream.device != device:
             stack.close()
             raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, device))

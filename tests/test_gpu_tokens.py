@@ -514,3 +514,29 @@ def test_gradients_on_offsets_out_of_order_or_range(rock, gpu, t, n, k, offsets)
     for e in range(E):
         want[at[e]:at[e + 1]] = (dout[at[e]:at[e + 1]].double() @ w[e].double()).to(TORCH[t])
     assert torch.equal(dx.cpu(), want)
+
+
+def test_the_default_stream_by_its_handle(rock, gpu):
+    """The raw handle of the default stream is 0: such a call is ordered with the work queued there, also while another
+    stream is the current one."""
+    _device_only(gpu)
+    import rocmlir_amd.api as api
+    default, side = torch.cuda.default_stream(gpu), torch.cuda.Stream(device=gpu)
+    assert default.cuda_stream == 0
+    g = generator(43)
+    src = torch.randn((4000, 2048), generator=g).half().to(gpu)
+    want_q, want_s = quantise64(src)
+    x, big = torch.zeros_like(src), torch.randn((4096, 4096), generator=g).to(gpu)
+    torch.cuda.synchronize()
+    for given in (0, default):
+        with torch.cuda.stream(side):
+            with api._on("test", gpu, given):
+                assert torch.cuda.current_stream() == default
+        x.zero_()
+        for _ in range(4):
+            big @ big                  # the copy waits behind these
+        x.copy_(src)
+        with torch.cuda.stream(side):
+            q, s = rock.quantize_tokens(x, stream=given)
+        default.synchronize()
+        assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
