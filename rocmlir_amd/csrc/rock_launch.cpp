@@ -105,17 +105,19 @@ bool check_launch_args(Handle *h, void *const *pointers, int num_pointers) {
   }
   if (h->op == OP_TOKENS)
     need_aux = true; // no bias slot: every pointer is a tensor
-  // a conversion kernel reads and writes the tensors of its own map; the problem's optional ones may be missing
+  // a conversion kernel reads and writes the tensors of its own map and those in its parameter block, all of them; the
+  // problem's others may be missing
   auto touched = [&](int i) {
-    if (h->op != OP_RELAYOUT || h->ptr_map.empty())
-      return true;
+    for (const Handle::ParamPtr &pp : h->param_ptrs)
+      if (pp.source == i)
+        return true;
     for (const Handle::PtrSrc &m : h->ptr_map)
       if (m.source == i)
         return true;
-    return false;
+    return h->ptr_map.empty() && i < h->num_pointers;
   };
   for (int i = 0; i < num_pointers; ++i)
-    if (!pointers[i] && (i != aux_index || need_aux) && touched(i)) {
+    if (!pointers[i] && (h->op == OP_RELAYOUT ? touched(i) : i != aux_index || need_aux)) {
       set_error("launch: NULL tensor pointer");
       return false;
     }
