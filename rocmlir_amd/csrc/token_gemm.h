@@ -416,14 +416,17 @@ template <int DT, int COLS, int NT> struct AnyCols {
     static constexpr int ES = Kg::ES, EPC = kChunk / ES, NCH = COLS * kRowBytes / kChunk / NT;
     static_assert(COLS * kRowBytes % (kChunk * NT) == 0, "whole chunks per thread");
   };
-  const char *base;
-  int64_t pitch; // bytes between consecutive k
-  int at[Gm::NCH], beyond[Gm::NCH]; // byte of a row where a lane's chunk is loaded from, elements it is moved down by
-  int cols, K, tid;
+  const char *base; // the tile's first column
+  int64_t pitch;    // bytes between consecutive k
+  // byte where a lane's chunk is loaded from, counted from the tile's first column (rows may be longer than 2 GiB; a
+  // chunk moved back from the row's end may start in front of the tile), elements it is moved down by
+  int at[Gm::NCH], beyond[Gm::NCH];
+  int first, cols, K, tid;
   bool edge; // some lane's chunk is moved
   __device__ __forceinline__ void init(const void *b, int64_t, int64_t ks, int col0, int c, int K_, int t) {
-    base = (const char *)b;
+    base = (const char *)b + (int64_t)col0 * Gm::ES;
     pitch = ks * Gm::ES;
+    first = col0;
     cols = c;
     K = K_;
     tid = t;
@@ -431,7 +434,7 @@ template <int DT, int COLS, int NT> struct AnyCols {
 #pragma unroll
     for (int i = 0; i < Gm::NCH; ++i) {
       const int col = col0 + (((t + i * NT) % Kg::CPR) ^ Kg::swz(krow(i))) * Gm::EPC, from = max(min(col, c - Gm::EPC), 0);
-      at[i] = from * Gm::ES;
+      at[i] = (from - col0) * Gm::ES;
       beyond[i] = min(col - from, Gm::EPC);
     }
   }
@@ -448,7 +451,7 @@ template <int DT, int COLS, int NT> struct AnyCols {
   __device__ __forceinline__ void load_elements(int kt, v4i (&r)[Gm::NCH]) const {
 #pragma unroll
     for (int i = 0; i < Gm::NCH; ++i) {
-      r[i] = tail_chunk<DT>(row(kt, i) + at[i] + beyond[i] * Gm::ES, at[i] / Gm::ES + beyond[i], cols);
+      r[i] = tail_chunk<DT>(row(kt, i) + at[i] + beyond[i] * Gm::ES, first + at[i] / Gm::ES + beyond[i], cols);
       if (kt * Kg::KR + krow(i) >= K)
         r[i] = v4i{0, 0, 0, 0};
     }

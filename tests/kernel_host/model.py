@@ -156,7 +156,8 @@ def build_model(d, types=(0, 1), rolled=False, attention=True, tokens=()):
     for name, text in units.items():
         with open(os.path.join(d, name + ".cpp"), "w") as f:
             f.write(text)
-    flags = [CLANG, "-O1", "-std=c++17", "-fPIC", "-w", "-I", HOST, "-I", CSRC]
+    # (-fwrapv: a position that passes 31 bits wraps as it does in the device's registers)
+    flags = [CLANG, "-O1", "-std=c++17", "-fPIC", "-fwrapv", "-w", "-I", HOST, "-I", CSRC]
     todo = [(os.path.join(d, n + ".cpp"), os.path.join(d, n + ".o")) for n in units]
     todo.append((os.path.join(HOST, "runner.cpp"), os.path.join(d, "runner.o")))
     running, limit = [], max(2, os.cpu_count() or 2)

@@ -540,3 +540,25 @@ def test_the_default_stream_by_its_handle(rock, gpu):
             q, s = rock.quantize_tokens(x, stream=given)
         default.synchronize()
         assert torch.equal(q.cpu(), want_q) and torch.equal(s.cpu(), want_s)
+
+
+@pytest.mark.parametrize("t", ["f16", "f32"])
+def test_single_rows_longer_than_two_gibibytes(rock, gpu, t):
+    """Columns whose byte position in their row passes 2^31, of weights stored [K, N] and of activations (every address
+    checked on the CPU build of the kernels first, tests/test_token_ops_model.py)."""
+    _device_only(gpu)
+    es = 2 if t == "f16" else 4
+    wide, depth, g = (1 << 31) // es + 203, 9, generator(47)
+    places = [slice(0, 300), slice(wide // 2 - 150, wide // 2 + 150), slice(wide - 203 - 300, wide - 203), slice(wide - 300, wide)]
+    long_rows = torch.zeros((depth, wide), dtype=TORCH[t], device=gpu)
+    for p in places:
+        long_rows[:, p] = whole(g, -3, 3, depth, 300).to(TORCH[t]).to(gpu)
+    x = whole(g, -3, 3, 2, depth).to(TORCH[t])
+    y = rock.grouped_gemm(x.to(gpu), long_rows[None], torch.tensor([0, 2], dtype=torch.int32, device=gpu))
+    dy = whole(g, -3, 3, depth, 9).to(TORCH[t])
+    dw = rock.grouped_gemm_bwd_weight(long_rows, dy.to(gpu), torch.tensor([0, depth], dtype=torch.int32, device=gpu))
+    for p in places:
+        cols = long_rows[:, p].cpu().double()
+        assert torch.equal(y[:, p].cpu().double(), x.double() @ cols), p
+        assert torch.equal(dw[0, p].cpu().double(), cols.t() @ dy.double()), p
+    assert not y[:, 300:700].any() and not dw[0, 300:700].any()

@@ -1,6 +1,7 @@
 """The kernels over token rows (csrc/token_gemm.h, csrc/quantize_tokens.hip) built for the CPU and run through whole
 plans: every address checked, loads landing at issue or at their wait, no byte written by two blocks, and on
 integer-valued data results equal to numpy's bit for bit.  The plans come from the C ABI as a caller gets them."""
+import ctypes as C
 import os
 import sys
 
@@ -8,7 +9,7 @@ import numpy as np
 import pytest
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-from tests.kernel_host.model import CLANG, build_model, run_plan  # noqa: E402
+from tests.kernel_host.model import CLANG, build_model, pointer_map, run_plan  # noqa: E402
 
 pytestmark = pytest.mark.skipif(CLANG is None, reason="the host build uses clang's vector extensions")
 
@@ -374,3 +375,56 @@ def test_gradients_on_offsets_that_step_back(model, rock, offsets, n, k, perf):
         assert np.array_equal(dx[a:b].astype(np.float64), dout[a:b].astype(np.float64) @ w[e].astype(np.float64)), (names, e)
         owned[a:b] = True
     assert (dx[~owned].view(np.uint8) == 0xEE).all()
+
+
+class _Sparse:
+    """A tensor whose pages exist where they are touched only."""
+
+    def __init__(self, nbytes):
+        import mmap
+        noreserve = 0x4000
+        self.map = mmap.mmap(-1, nbytes, flags=mmap.MAP_SHARED | mmap.MAP_ANONYMOUS | noreserve)
+        self.bytes = np.frombuffer(self.map, np.uint8)
+        self.at = self.bytes.ctypes.data
+
+    def of(self, dtype, shape):
+        return self.bytes[:int(np.prod(shape, dtype=np.int64)) * np.dtype(dtype).itemsize].view(dtype).reshape(shape)
+
+
+@pytest.mark.parametrize("depth", [1, 9], ids=["elements", "chunks"])
+@pytest.mark.parametrize("op,t", [("grouped_gemm", "f16"), ("grouped_gemm", "f32"), ("grouped_gemm_bwd_weight", "f16")])
+def test_rows_longer_than_two_gibibytes(model, rock, op, t, depth):
+    """Columns whose byte position in their row passes 2^31, in K-major operands of any alignment: the last two tiles of a
+    launch, on tensors that are mostly holes."""
+    weight, ty = op != "grouped_gemm", _NUMPY[t]
+    es = np.dtype(ty).itemsize
+    wide, rows = (1 << 31) // es + 203, 9 if weight else 2
+    # product: x [rows, depth] times w [depth, wide]; weight gradient: x [depth, wide], dout [depth, rows] -> [wide, rows]
+    opts = _opts(op, t, *((depth, 1, rows, wide) if weight else (rows, 1, wide, depth)), False, "-perf_config v2:128,128")
+    k = rock.RockKernel(opts)
+    assert "_128x128_any" in k.kernel_name and k.block_size == 256
+    tensors = [_Sparse(int(np.prod(dims, dtype=np.int64)) * 4 + 4096) for _, dims in k.arguments()]
+    rng = np.random.default_rng(depth)
+    small = rng.integers(-3, 4, (depth, rows) if weight else (rows, depth)).astype(ty)
+    wide_tensor = tensors[0 if weight else 1].of(ty, (depth, wide))
+    tail = 75 + 128                                            # columns of the last two tiles
+    wide_tensor[:, -tail - 40:] = rng.integers(-3, 4, (depth, tail + 40))
+    tensors[2 if weight else 0].of(ty, small.shape)[:] = small
+    tensors[3].of(np.int32, (2,))[:] = [0, depth if weight else rows]
+    ptrs = (C.c_void_p * 8)()
+    for j, (src, off) in enumerate(pointer_map(rock, k)):
+        ptrs[j] = None if src < 0 else tensors[src].at + off
+    text = C.create_string_buffer(512)
+    model.hm_clear()
+    model.hm_set_blocks(k.grid_size - 2, 2)
+    try:
+        bad = model.hm_run(k.kernel_name.encode(), k.params(), ptrs, k.grid_size, k.block_size, text, 512)
+    finally:
+        model.hm_set_blocks(0, 0xFFFFFFFF)
+    assert bad == 0, text.value
+    columns = wide_tensor[:, -tail:].astype(np.float64)
+    if weight:
+        got, want = tensors[1].of(ty, (wide, rows))[-tail:], columns.T @ small.astype(np.float64)
+    else:
+        got, want = tensors[2].of(ty, (rows, wide))[:, -tail:], small.astype(np.float64) @ columns
+    assert np.array_equal(got.astype(np.float64), want)
