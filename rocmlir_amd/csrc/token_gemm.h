@@ -16,6 +16,7 @@ namespace rk {
 // ---- parameter blocks of a tile -----------------------------------------------------------
 struct TokenTileParams : RockGemmParams {};
 // results are f32, f16 or bf16
+template <int OD> constexpr bool kTokenResult = OD == ROCK_F32 || OD == ROCK_F16 || OD == ROCK_BF16;
 template <bool INT_ACC, typename F>
 __device__ __forceinline__ void dispatch_tile_dtype(const TokenTileParams &p, F &&f) {
   switch (p.epi.out_dtype) {
@@ -32,6 +33,11 @@ struct TokenScaleParams : TokenTileParams {
   const float *token_scale;   // of the tile's group: element m belongs to row m
   const float *channel_scale; // element n to column n; NULL: epi.scale
 };
+// (of its own: for a derived block the template over any parameter block would be the better match)
+template <bool INT_ACC, typename F>
+__device__ __forceinline__ void dispatch_tile_dtype(const TokenScaleParams &p, F &&f) {
+  dispatch_tile_dtype<INT_ACC>(static_cast<const TokenTileParams &>(p), static_cast<F &&>(f));
+}
 __device__ __forceinline__ float token_scale_of(const TokenScaleParams &p, int m) {
   return p.token_scale && m < p.M ? p.token_scale[m] : 1.0f;
 }
@@ -48,6 +54,7 @@ __device__ __forceinline__ float scaled_value(int sum, float zero_point, float s
 // four channels of row m, packed in the result's type
 template <int OD>
 __device__ __forceinline__ v4i token_convert4(const v4i &acc, const TokenScaleParams &p, int m, const void *bias, int n0) {
+  static_assert(kTokenResult<OD>, "dispatch_tile_dtype must pick the list of these kernels");
   const RockEpilogue &e = p.epi;
   const float t = token_scale_of(p, m);
   float v[4];
@@ -67,8 +74,8 @@ __device__ __forceinline__ v4i token_convert4(const v4f &acc, const TokenTilePar
 // Epilogue of the tiled kernels with these scales.  The raw sums go through the wave's LDS region, 32 rows at a time,
 // and are scaled on the way out, where a lane holds eight consecutive columns of one row: its channel scales and biases
 // are then the same for all its rows and are loaded once.  Scaled where they sit in the accumulators, every group of
-// four would load its own, behind a bounds test each, three output types over: four minutes of compilation and a hundred
-// spilled scalar registers in the 256 x 256 tile.
+// four would load its own, behind a bounds test each, once for every output type: four minutes of compilation and a
+// hundred spilled scalar registers in the 256 x 256 tile (measured with seven types; it has three).
 template <> struct HasRowScales<TokenScaleParams> : std::true_type {};
 template <int DT, int MI, int NI, int NWAVES, int LDS_BYTES, typename Params>
 __device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (&acc)[MI][NI], const Params &p, int g,
@@ -93,6 +100,7 @@ __device__ __forceinline__ void row_scale_epilogue(typename MmaTraits<DT>::Acc (
   __builtin_amdgcn_s_barrier(); // every wave is done reading the operand stages
   dispatch_tile_dtype<true>(p, [&](auto od_const) __attribute__((always_inline)) {
     constexpr int OD = decltype(od_const)::value, ES = OutElemSize<OD>::value;
+    static_assert(kTokenResult<OD>, "dispatch_tile_dtype must pick the list of these kernels");
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
 #pragma unroll
