@@ -986,16 +986,18 @@ def _on(name, device, stream):
 
 
 def _result(name, out, shape, dtype, like, *operands):
-    """`out` checked, or a new tensor on `like`'s device."""
+    """`out` checked, or a new tensor on `like`'s device.  `operands`: whatever else the call reads or writes."""
     if out is None:
         return like.new_empty(shape, dtype=dtype)
     begin, end = out.data_ptr(), out.data_ptr() + out.nbytes
     for t in (like,) + operands:
+        if t is None:
+            continue
         span = t.nbytes   # with strides: from the first to the last element
         if not t.is_contiguous() and span:
             span = (sum((n - 1) * st for n, st in zip(t.shape, t.stride())) + 1) * t.element_size()
         if begin < t.data_ptr() + span and t.data_ptr() < end:
-            raise RockError("%s: out overlaps an operand" % name)
+            raise RockError("%s: a result overlaps an operand or another result" % name)
     if tuple(out.shape) != tuple(shape) or out.dtype != dtype or out.device != like.device:
         raise RockError("%s: out must be %s of %s on %s" % (name, tuple(shape), dtype, like.device))
     if not out.is_contiguous() or out.data_ptr() & 15:
@@ -1034,7 +1036,7 @@ def quantize_tokens(x, *, out=None, scale_out=None, stream=None, info=None):
         with _on(name, x.device, stream):
             return quantize_tokens(x, out=out, scale_out=scale_out, info=info)
     q = _result(name, out, shape, torch.int8, x)
-    s = _result(name, scale_out, shape[:-1], torch.float32, x)
+    s = _result(name, scale_out, shape[:-1], torch.float32, x, q)
     count, cols = x.numel(), shape[-1]
     if count == 0:
         return q, s.zero_()   # rows without elements: their largest magnitude is 0
@@ -1071,7 +1073,8 @@ def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, a
                _scale_vector(name, "token_scale", token_scale, M)]
     if vector:
         tensors.append(_scale_vector(name, "scale", scale, N))
-    res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a, b)
+    res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a, b, token_scale,
+                               scale if vector else None, bias)
     if M == 0:
         return res
     lo, hi = (None, None) if clip is None else (float(clip[0]), float(clip[1]))
@@ -1136,7 +1139,8 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
         tensors.append(_scale_vector(name, "token_scale", token_scale, T))
     if vector:
         tensors.append(_scale_vector(name, "scale", scale, E * N))
-    res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x, w, offsets)
+    res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x, w, offsets, token_scale,
+                               scale if vector else None)
     if T == 0 or N == 0:
         return res
     prog = _token_plan("operation t g m n k transB out_datatype token_scale_vector scale_vector scale perf_config", name, t,

@@ -106,3 +106,36 @@ def test_tuning_space_of_the_new_operators(rock):
     for perf in space:
         assert rock.RockKernel(k.options + " -perf_config " + perf).perf_config == perf
     assert len(rock.RockKernel("-operation quantize_tokens -t f16 -m 5 -k 8").tuning_space()) == 1
+
+
+def _i8_gemm(r, **kw):
+    return r.gemm(_t(4, 16, dtype=I8), _t(4, 16, dtype=I8), transB=True, out_dtype="f32", **dict(dict(token_scale=torch.ones(4)), **kw))
+
+
+def _i8_grouped(r, **kw):
+    return r.grouped_gemm(_t(4, 16, dtype=I8), _t(1, 4, 16, dtype=I8), OFF3[:2], transB=True, out_dtype="f32", **kw)
+
+
+@pytest.mark.parametrize("call", [
+    lambda r, b: _i8_gemm(r, out=b[:16].view(4, 4), token_scale=b[12:16]),
+    lambda r, b: _i8_gemm(r, out=b[:16].view(4, 4), scale=b[4:8]),
+    lambda r, b: _i8_gemm(r, out=b[:16].view(4, 4), bias=b[:4]),
+    lambda r, b: _i8_grouped(r, out=b[:16].view(4, 4), token_scale=b[12:16]),
+    lambda r, b: _i8_grouped(r, out=b[:16].view(4, 4), scale=b[4:8].view(1, 4)),
+    lambda r, b: _i8_grouped(r, out=b[:16].view(4, 4), token_scale=b[13:30:5]),       # (copied first, refused all the same)
+    lambda r, b: r.quantize_tokens(_t(4, 16), out=b.view(I8)[:64].view(4, 16), scale_out=b[12:16]),
+    lambda r, b: r.quantize_tokens(b[:16].view(4, 4), scale_out=b[12:16]),
+])
+def test_results_may_not_overlap_scales_or_each_other(rock, call):
+    with pytest.raises(rock.RockError, match="overlaps"):
+        call(rock, torch.zeros(64))
+
+
+def test_results_beside_scales_are_taken(rock):
+    """The same tensors without the overlap get as far as the device check."""
+    b = torch.zeros(64)
+    for call in (lambda: _i8_gemm(rock, out=b[:16].view(4, 4), token_scale=b[16:20], scale=b[20:24], bias=b[24:28]),
+                 lambda: _i8_grouped(rock, out=b[:16].view(4, 4), token_scale=b[16:20], scale=b[20:24].view(1, 4)),
+                 lambda: rock.quantize_tokens(b[32:].view(4, 8), out=b.view(I8)[:32].view(4, 8), scale_out=b[8:12])):
+        with pytest.raises(rock.RockError, match="must live on the GPU"):
+            call()
