@@ -985,6 +985,13 @@ def _on(name, device, stream):
     return stack
 
 
+def _depth_of_one(rows, weights, axis):
+    """Operands of a product over no depth as ones of depth 1 (`axis` of the weights) that hold zeros: the same sums."""
+    shape = list(weights.shape)
+    shape[axis] = 1
+    return rows.new_zeros(rows.shape[:-1] + (1,)), weights.new_zeros(shape)
+
+
 def _result(name, out, shape, dtype, like, *operands):
     """`out` checked, or a new tensor on `like`'s device.  `operands`: whatever else the call reads or writes."""
     if out is None:
@@ -1075,8 +1082,11 @@ def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, a
         tensors.append(_scale_vector(name, "scale", scale, N))
     res = tensors[2] = _result(name, out, (M, N) if a.dim() == 2 else (1, M, N), _torch_dtype(out_dtype), a, b, token_scale,
                                scale if vector else None, bias)
-    if M == 0:
+    if M == 0 or N == 0:
         return res
+    if K == 0:
+        K = 1
+        tensors[0], tensors[1] = _depth_of_one(a, b, -1 if transB else -2)
     lo, hi = (None, None) if clip is None else (float(clip[0]), float(clip[1]))
     prog = _token_plan("operation t token_scale_vector m n k transB out_datatype scale_vector scale zero_point bias "
                        "activation clip_min clip_max perf_config", "gemm", "i8", True, M, N, K, bool(transB), out_dtype,
@@ -1143,6 +1153,9 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
                                scale if vector else None)
     if T == 0 or N == 0:
         return res
+    if K == 0:
+        K = 1
+        tensors[0], tensors[1] = _depth_of_one(x, w, 2 if transB else 1)
     prog = _token_plan("operation t g m n k transB out_datatype token_scale_vector scale_vector scale perf_config", name, t,
                        E, T, N, K, bool(transB), out_dtype, token_scale is not None, vector,
                        None if vector or scale is None else float(scale), perf_config)
@@ -1168,6 +1181,9 @@ def grouped_gemm_bwd_data(dout, w, offsets, *, transB=False, out=None, stream=No
     res = _result(name, out, (T, K), dout.dtype, dout, w, offsets)
     if T == 0 or K == 0:
         return res
+    if N == 0:
+        N = 1
+        dout, w = _depth_of_one(dout, w, 1 if transB else 2)
     prog = _token_plan("operation t g m n k transB perf_config", name, t, E, T, N, K, bool(transB), perf_config)
     _launch_tokens(prog, info, res, _dense(w), _dense(dout), _dense(offsets))
     return res

@@ -562,3 +562,29 @@ def test_single_rows_longer_than_two_gibibytes(rock, gpu, t):
         assert torch.equal(y[:, p].cpu().double(), x.double() @ cols), p
         assert torch.equal(dw[0, p].cpu().double(), cols.t() @ dy.double()), p
     assert not y[:, 300:700].any() and not dw[0, 300:700].any()
+
+
+@pytest.mark.parametrize("transB", [True, False], ids=["NK", "KN"])
+def test_a_reduction_over_nothing(rock, gpu, transB):
+    """K = 0 (N = 0 in the gradient of the rows): sums of nothing are 0, the epilogue is applied to them, and rows of no
+    expert stay as they were.  What quantize_tokens returns for rows without elements goes through the products."""
+    off = make_offsets([2, 0, 3]).to(gpu)
+    x = torch.empty((7, 0), dtype=torch.bfloat16, device=gpu)
+    w = torch.empty((3, 6, 0) if transB else (3, 0, 6), dtype=torch.bfloat16, device=gpu)
+    y = torch.full((7, 6), -7.0, dtype=torch.bfloat16, device=gpu)
+    rock.grouped_gemm(x, w, off, transB=transB, out=y)
+    assert (y[:5] == 0).all() and (y[5:] == -7).all()
+    wd = torch.empty((3, 0, 6) if transB else (3, 6, 0), dtype=torch.bfloat16, device=gpu)
+    dx = torch.full((7, 6), -7.0, dtype=torch.bfloat16, device=gpu)
+    rock.grouped_gemm_bwd_data(x, wd, off, transB=transB, out=dx)
+    assert (dx[:5] == 0).all() and (dx[5:] == -7).all()
+    q, s = rock.quantize_tokens(x)
+    assert q.shape == (7, 0) and (s == 0).all()
+    wq = torch.empty((3, 6, 0) if transB else (3, 0, 6), dtype=torch.int8, device=gpu)
+    y = torch.full((7, 6), -7.0, dtype=torch.float16, device=gpu)
+    rock.grouped_gemm(q, wq, off, transB=transB, token_scale=s, scale=torch.ones((3, 6), device=gpu), out=y)
+    assert (y[:5] == 0).all() and (y[5:] == -7).all()
+    token, bias = torch.tensor([1.0, 2.0, 3.0, 4.0, 5.0, 6.0, float("nan")], device=gpu), torch.arange(6.0, device=gpu)
+    y = rock.gemm(q, wq[0], transB=transB, token_scale=token, scale=0.5, zero_point=3, bias=bias, out_dtype="f32")
+    want = -1.5 * token[:, None] + bias
+    assert torch.equal(y[:6], want[:6]) and y[6].isnan().all()

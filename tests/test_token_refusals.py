@@ -139,3 +139,35 @@ def test_results_beside_scales_are_taken(rock):
                  lambda: rock.quantize_tokens(b[32:].view(4, 8), out=b.view(I8)[:32].view(4, 8), scale_out=b[8:12])):
         with pytest.raises(rock.RockError, match="must live on the GPU"):
             call()
+
+
+def test_an_empty_dimension_of_the_result_is_an_empty_result(rock):
+    """Nothing to compute: the (empty) result, checked like any other."""
+    e8 = torch.zeros((0, 16), dtype=I8)
+    assert rock.gemm(_t(4, 16, dtype=I8), e8, transB=True, token_scale=torch.ones(4)).shape == (4, 0)
+    assert rock.gemm(_t(4, 16, dtype=I8), e8.t(), token_scale=torch.ones(4), out_dtype="f32").dtype == torch.float32
+    assert rock.gemm(e8, _t(6, 16, dtype=I8), transB=True, token_scale=torch.ones(0), bias=torch.ones(6)).shape == (0, 6)
+    assert rock.grouped_gemm(_t(5, 8), _t(3, 0, 8), OFF3, transB=True).shape == (5, 0)
+    assert rock.grouped_gemm(_t(5, 0), _t(3, 0, 0), OFF3).shape == (5, 0)
+    assert rock.grouped_gemm(_t(0, 0), _t(3, 0, 6), OFF3).shape == (0, 6)
+    assert rock.grouped_gemm_bwd_data(_t(5, 6), _t(3, 6, 0), OFF3, transB=True).shape == (5, 0)
+    assert rock.grouped_gemm_bwd_data(_t(0, 0), _t(3, 0, 8), OFF3, transB=True).shape == (0, 8)
+    assert rock.grouped_gemm_bwd_weight(_t(5, 0), _t(5, 6), OFF3).shape == (3, 0, 6)
+    with pytest.raises(rock.RockError, match="token_scale must hold 4"):
+        rock.gemm(_t(4, 16, dtype=I8), e8, transB=True, token_scale=torch.ones(3))
+    with pytest.raises(rock.RockError, match="out must be"):
+        rock.grouped_gemm(_t(5, 8), _t(3, 0, 8), OFF3, transB=True, out=_t(5, 1))
+
+
+@pytest.mark.parametrize("call", [
+    lambda r: r.gemm(_t(4, 0, dtype=I8), _t(6, 0, dtype=I8), transB=True, token_scale=torch.ones(4)),
+    lambda r: r.gemm(_t(4, 0, dtype=I8), _t(0, 6, dtype=I8), token_scale=torch.ones(4)),
+    lambda r: r.grouped_gemm(_t(5, 0), _t(3, 6, 0), OFF3, transB=True),
+    lambda r: r.grouped_gemm(_t(5, 0, dtype=I8), _t(3, 0, 6, dtype=I8), OFF3),
+    lambda r: r.grouped_gemm_bwd_data(_t(5, 0), _t(3, 0, 8), OFF3, transB=True),
+    lambda r: r.grouped_gemm_bwd_data(_t(5, 0), _t(3, 8, 0), OFF3),
+])
+def test_an_empty_reduction_is_a_product(rock, call):
+    """Not refused for its depth: it gets as far as the device check."""
+    with pytest.raises(rock.RockError, match="must live on the GPU"):
+        call(rock)
