@@ -91,8 +91,9 @@ typedef void *MiirHandle;
  *     x [m,k] times the weights [g,k,n] ([g,n,k] with transB) of the group whose
  *     range [offsets[e], offsets[e+1]) holds it; pointers x, weights, result,
  *     offsets int32 [g+1] in device memory, [token scales [m]], [channel scales
- *     [g,n]].  Rows of no group are not written; an offset that steps back or
- *     lies outside [0, m] is read as the furthest one before it;
+ *     [g,n]].  Rows of no group are not written.  An offset below 0 is read as
+ *     0, one beyond m as m, and one that steps back as the furthest one before
+ *     it, in the product and in both gradients;
  *   grouped_gemm_bwd_data, grouped_gemm_bwd_weight: its gradients, with its keys
  *     and pointer order, the gradient written in its own slot (weights of a
  *     group without rows: zeros).

@@ -1120,8 +1120,8 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
                  perf_config=None, info=None):
     """Products grouped by expert: rows offsets[e] <= t < offsets[e + 1] of x [T, K] times w[e], w [E, K, N]
     ([E, N, K] if transB) -> [T, N].  `offsets` is int32 [E + 1] on the GPU, never read on the host: non-decreasing
-    values within [0, T] (an offset that steps back or lies outside is taken as the furthest one before it).  Experts
-    may have no rows; rows of no expert are not written: they keep what `out` held (undefined without `out`).  f16,
+    values within [0, T] (one below 0 is taken as 0, one beyond T as T, one that steps back as the furthest one before
+    it).  Experts may have no rows, K may be 0 (sums of nothing are 0); rows of no expert are not written: they keep what `out` held (undefined without `out`).  f16,
     bf16 and f32 operands give a result of their type unless `out_dtype` names another of the three; int8 operands
     give sum * scale * token_scale as f16 (default), bf16 or f32, `token_scale` float32 [T], `scale` float32 [E, N] or
     a number (both optional)."""

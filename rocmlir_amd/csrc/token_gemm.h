@@ -148,7 +148,7 @@ struct GroupTile {
 
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_ds_bpermute(lane * 4, v); }
 
-// Boundaries that step back or lie outside [0, M] are read as if they stood at the furthest boundary before them, so
+// Boundaries are clamped to [0, M], and one that steps back is read as if it stood at the furthest one before it, so
 // that whatever the offsets hold the groups are disjoint ranges of the M rows and every row tile is counted once.
 struct GroupScan {
   int end, tiles; // running over the groups seen so far

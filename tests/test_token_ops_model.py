@@ -428,3 +428,20 @@ def test_rows_longer_than_two_gibibytes(model, rock, op, t, depth):
     else:
         got, want = tensors[2].of(ty, (rows, wide))[:, -tail:], small.astype(np.float64) @ columns
     assert np.array_equal(got.astype(np.float64), want)
+
+
+def test_offsets_beyond_the_rows_are_clamped(model, rock):
+    """As the header and grouped_gemm() say: below 0 is 0, beyond the rows is their number, stepping back is the furthest
+    one before.  [-4, 2, 100, 7] over 12 rows: group 0 has the rows 0 and 1, group 1 the rest, group 2 none."""
+    T, n, k = 12, 24, 32
+    x, w = np.ones((T, k), np.float16), np.stack([np.full((n, k), v, np.float16) for v in (1, 2, 3)])
+    off = np.array([-4, 2, 100, 7], np.int32)
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm", "f16", T, 3, n, k, True), {0: x, 1: w, 3: off})
+    assert not problems, (names, problems)
+    res = got[2][:T * n * 2].view(np.float16).reshape(T, n)
+    assert (res[:2] == k).all() and (res[2:] == 2 * k).all()
+    names, problems, got = run_plan(model, rock, _opts("grouped_gemm_bwd_weight", "f16", T, 3, n, k, True),
+                                    {0: x, 2: np.ones((T, n), np.float16), 3: off})
+    assert not problems, (names, problems)
+    dw = got[1][:w.nbytes].view(np.float16).reshape(w.shape)
+    assert (dw[0] == 2).all() and (dw[1] == 10).all() and (dw[2] == 0).all()
