@@ -1121,10 +1121,10 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
     """Products grouped by expert: rows offsets[e] <= t < offsets[e + 1] of x [T, K] times w[e], w [E, K, N]
     ([E, N, K] if transB) -> [T, N].  `offsets` is int32 [E + 1] on the GPU, never read on the host: non-decreasing
     values within [0, T] (one below 0 is taken as 0, one beyond T as T, one that steps back as the furthest one before
-    it).  Experts may have no rows, K may be 0 (sums of nothing are 0); rows of no expert are not written: they keep what `out` held (undefined without `out`).  f16,
-    bf16 and f32 operands give a result of their type unless `out_dtype` names another of the three; int8 operands
-    give sum * scale * token_scale as f16 (default), bf16 or f32, `token_scale` float32 [T], `scale` float32 [E, N] or
-    a number (both optional)."""
+    it).  Experts may have no rows, K may be 0 (sums of nothing are 0); rows of no expert are not written: they keep
+    what `out` held (undefined without `out`).  f16, bf16 and f32 operands give a result of their type unless
+    `out_dtype` names another of the three; int8 operands give sum * scale * token_scale as f16 (default), bf16 or f32,
+    `token_scale` float32 [T], `scale` float32 [E, N] or a number (both optional)."""
     if torch is None:
         _load_torch()
     name = "grouped_gemm"
@@ -1149,6 +1149,8 @@ def grouped_gemm(x, w, offsets, *, transB=False, out_dtype=None, token_scale=Non
         tensors.append(_scale_vector(name, "token_scale", token_scale, T))
     if vector:
         tensors.append(_scale_vector(name, "scale", scale, E * N))
+        if scale.dim() > 1 and [d for d in scale.shape if d != 1] != [d for d in (E, N) if d != 1]:
+            raise RockError("%s: scale is [E, N], not %s" % (name, list(scale.shape)))
     res = tensors[2] = _result(name, out, (T, N), _torch_dtype(out_dtype), x, w, offsets, token_scale,
                                scale if vector else None)
     if T == 0 or N == 0:

@@ -171,3 +171,11 @@ def test_an_empty_reduction_is_a_product(rock, call):
     """Not refused for its depth: it gets as far as the device check."""
     with pytest.raises(rock.RockError, match="must live on the GPU"):
         call(rock)
+
+
+@pytest.mark.parametrize("shape,taken", [((3, 6), True), ((3, 1, 6), True), ((3, 6, 1), True), ((18,), True), ((6, 3), False), ((2, 9), False),
+                                         ((3, 2, 3), False), ((1, 6, 3), False)])
+def test_channel_scales_of_experts_in_another_order(rock, shape, taken):
+    """[E, N], with dimensions of one anywhere, or flat; as many values in another order are not what the caller means."""
+    with pytest.raises(rock.RockError, match="must live on the GPU" if taken else "scale is .E, N."):
+        rock.grouped_gemm(_t(5, 16, dtype=I8), _t(3, 6, 16, dtype=I8), OFF3, transB=True, scale=torch.ones(shape))
