@@ -588,3 +588,47 @@ def test_a_reduction_over_nothing(rock, gpu, transB):
     y = rock.gemm(q, wq[0], transB=transB, token_scale=token, scale=0.5, zero_point=3, bias=bias, out_dtype="f32")
     want = -1.5 * token[:, None] + bias
     assert torch.equal(y[:6], want[:6]) and y[6].isnan().all()
+
+
+# (rows per expert, N, K): 256 x 256 tiles of the product, of the gradient of the rows and of the weights'
+ROUNDS = [([300, 1, 0, 2000, 513, 256, 40, 700], 4064, 4112, "quarters"),    # 19 row tiles x 16: 256 + 48; x 17: 256 + 67 (halves)
+          ([300, 1, 0, 2000, 513, 256, 40, 700], 4592, 4096, "halves"),      # x 18: 256 + 86; x 16: 256 + 48 (quarters)
+          ([700, 0, 33], 2832, 3600, "weights")]                             # 3 x 12 x 15: 512 + 28; dW alone passes a round
+
+
+@pytest.mark.parametrize("t", ["bf16", "i8"])
+@pytest.mark.parametrize("transB", [True, False], ids=["NK", "KN"])
+@pytest.mark.parametrize("sizes,n,k,which", ROUNDS, ids=[r[3] for r in ROUNDS])
+def test_whole_rounds_of_tiles_and_then_parts(rock, gpu, sizes, n, k, which, transB, t):
+    """More 256 x 256 tiles than compute units: whole rounds of them, then what is left in quarters (up to 64 tiles) or in
+    halves (up to 128), in the product, the gradient of the rows and the gradient of the weights."""
+    _device_only(gpu)
+    tiles = lambda c: -(-c // 256)   # noqa: E731
+    rows, E, T = sum(tiles(s) for s in sizes), len(sizes), sum(sizes)
+    of_products, of_weights = (rows * tiles(n), rows * tiles(k)), E * tiles(n) * tiles(k)
+    counted = of_products if which != "weights" else (of_weights,)
+    assert all(c > 256 and 0 < c % 256 <= 128 for c in counted), (of_products, of_weights)
+    assert which == "weights" or {c % 256 <= 64 for c in counted} == {True, False}     # quarters in one, halves in the other
+    kind, g = torch.int8 if t == "i8" else TORCH[t], torch.Generator(device=gpu)
+    g.manual_seed(n)
+    # 40 columns of x and of dout are not 0, so that the 64-bit products here stay short; they sum exactly
+    some_k, some_n = (torch.randperm(c, generator=generator(c))[:40].sort().values.to(gpu) for c in (k, n))
+    x, dout = torch.zeros((T, k), dtype=kind, device=gpu), torch.zeros((T, n), dtype=kind, device=gpu)
+    x[:, some_k] = torch.randint(-2, 3, (T, 40), generator=g, device=gpu).to(kind)
+    dout[:, some_n] = torch.randint(-2, 3, (T, 40), generator=g, device=gpu).to(kind)
+    w = torch.randint(-1, 2, (E, n, k), generator=g, device=gpu, dtype=torch.int8).to(kind)
+    wd, off = (w if transB else w.transpose(1, 2).contiguous()), make_offsets(sizes).to(gpu)
+    info, kw = {}, dict(transB=transB, perf_config="v2:256,256")
+    y = rock.grouped_gemm(x, wd, off, out_dtype="f32" if t == "i8" else None, info=info, **kw)
+    assert "256x256_fast" in info["kernel_name"]
+    if t != "i8":
+        dx, dw = rock.grouped_gemm_bwd_data(dout, wd, off, **kw), rock.grouped_gemm_bwd_weight(x, dout, off, info=info, **kw)
+        assert info["kernel_name"].endswith("256x256")
+    for e, a, b in spans(sizes):
+        xe, de, we = x[a:b][:, some_k].double(), dout[a:b][:, some_n].double(), w[e].double()
+        assert torch.equal(y[a:b], (xe @ we[:, some_k].t()).to(y.dtype)), e
+        if t != "i8":
+            assert torch.equal(dx[a:b], (de @ we[some_n]).to(kind)), e
+            want = torch.zeros((n, k), dtype=torch.float64, device=gpu)
+            want[some_n[:, None], some_k] = de.t() @ xe
+            assert torch.equal(dw[e], (want if transB else want.t()).to(kind)), e
