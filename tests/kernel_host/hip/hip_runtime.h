@@ -91,6 +91,7 @@ template <typename T> inline T hm_readfirstlane(T v) { // (the kernels use it on
 #define __builtin_amdgcn_readfirstlane(x) hm_readfirstlane(x)
 #define __builtin_amdgcn_ballot_w64(x) hm_ballot(x)
 #define __builtin_amdgcn_ds_bpermute(a, v) hm_bpermute(a, v)
+#define __builtin_amdgcn_readlane(v, l) hm_bpermute((l) * 4, v)
 template <typename T> inline T __shfl_xor(T v, int mask, int width = 64) {
   hm_shuffle_xor(&v, sizeof v, mask, width);
   return v;
