@@ -957,6 +957,8 @@ def _dense(t):
 def _same_device(name, first, *others):
     index = first.get_device()      # (-1: the host's memory)
     for t in others:
+        if t is not None and not _is_tensor(t):
+            raise RockError("%s: %r is not a tensor" % (name, t))
         if t is not None and t.get_device() != index:
             raise RockError("%s: a tensor is on %s, the first operand on %s" % (name, t.device, first.device))
 
@@ -1100,7 +1102,7 @@ def _token_scaled_gemm(a, b, transB, out_dtype, scale, zero_point, bias, relu, a
 def _check_offsets(name, offsets, E):
     if E < 1:
         raise RockError("%s: no experts" % name)
-    if offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != E + 1:
+    if not _is_tensor(offsets) or offsets.dtype != torch.int32 or offsets.dim() != 1 or offsets.shape[0] != E + 1:
         raise RockError("%s: offsets is int32 [E + 1], the first row of every expert and the end of the last" % name)
 
 
@@ -1200,7 +1202,8 @@ def grouped_gemm_bwd_weight(x, dout, offsets, *, transB=False, out=None, stream=
     name = "grouped_gemm_bwd_weight"
     if x.dim() != 2 or dout.dim() != 2 or x.shape[0] != dout.shape[0] or x.dtype != dout.dtype:
         raise RockError("%s: x [T, K] and dout [T, N] of one type" % name)
-    E, T, K, N = offsets.shape[0] - 1 if offsets.dim() == 1 else 0, x.shape[0], x.shape[1], dout.shape[1]
+    E = offsets.shape[0] - 1 if _is_tensor(offsets) and offsets.dim() == 1 else 1   # (anything else is refused below)
+    T, K, N = x.shape[0], x.shape[1], dout.shape[1]
     _check_offsets(name, offsets, E)
     t = _dtype_name(x.dtype)
     if t not in ("f32", "f16", "bf16"):

@@ -179,3 +179,16 @@ def test_channel_scales_of_experts_in_another_order(rock, shape, taken):
     """[E, N], with dimensions of one anywhere, or flat; as many values in another order are not what the caller means."""
     with pytest.raises(rock.RockError, match="must live on the GPU" if taken else "scale is .E, N."):
         rock.grouped_gemm(_t(5, 16, dtype=I8), _t(3, 6, 16, dtype=I8), OFF3, transB=True, scale=torch.ones(shape))
+
+
+@pytest.mark.parametrize("call", [
+    lambda r: _i8_gemm(r, token_scale=0.5),
+    lambda r: _i8_gemm(r, bias=[1.0] * 4),
+    lambda r: _i8_grouped(r, token_scale=[1.0] * 4),
+    lambda r: r.grouped_gemm(_t(5, 8), _t(3, 6, 8), [0, 1, 2, 3], transB=True),
+    lambda r: r.grouped_gemm_bwd_data(_t(5, 6), _t(3, 6, 8), (0, 1, 2, 3), transB=True),
+    lambda r: r.grouped_gemm_bwd_weight(_t(5, 8), _t(5, 6), [0, 1, 2, 3]),
+])
+def test_what_must_be_a_tensor(rock, call):
+    with pytest.raises(rock.RockError, match="tensor|offsets is int32"):
+        call(rock)
