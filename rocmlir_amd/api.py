@@ -971,20 +971,22 @@ def _elsewhere(device, stream):
 def _on(name, device, stream):
     """A context that makes the operands' device the current one and `stream` (default: the device's current stream)
     torch's current stream, so that copies and results made on the way are ordered with the kernels."""
-    stack = contextlib.ExitStack()
     if device.type != "cuda":
-        return stack
-    stack.enter_context(torch.cuda.device(device))
-    if stream is not None:
-        if not isinstance(stream, torch.cuda.Stream):
-            handle = int(getattr(stream, "cuda_stream", stream))
-            # (handle 0 is the default stream; ExternalStream(0) would be one of torch's own, ordered with nothing)
-            stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
-        if stream.device != device:
-            stack.close()
-            raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, device))
-        stack.enter_context(torch.cuda.stream(stream))
-    return stack
+        return contextlib.ExitStack()
+    with contextlib.ExitStack() as stack:      # (left by an exception, it puts the device back)
+        stack.enter_context(torch.cuda.device(device))
+        if stream is not None:
+            if not isinstance(stream, torch.cuda.Stream):
+                try:
+                    handle = int(getattr(stream, "cuda_stream", stream))
+                except (TypeError, ValueError):
+                    raise RockError("%s: %r is no stream" % (name, stream))
+                # (handle 0 is the default stream; ExternalStream(0) would be one of torch's own, ordered with nothing)
+                stream = torch.cuda.ExternalStream(handle, device=device) if handle else torch.cuda.default_stream(device)
+            if stream.device != device:
+                raise RockError("%s: the stream is on %s, the tensors on %s" % (name, stream.device, device))
+            stack.enter_context(torch.cuda.stream(stream))
+        return stack.pop_all()
 
 
 def _depth_of_one(rows, weights, axis):

@@ -192,3 +192,26 @@ def test_channel_scales_of_experts_in_another_order(rock, shape, taken):
 def test_what_must_be_a_tensor(rock, call):
     with pytest.raises(rock.RockError, match="tensor|offsets is int32"):
         call(rock)
+
+
+def test_a_refused_stream_leaves_the_current_device(rock, monkeypatch):
+    """Whatever goes wrong with the stream of a call, the device that the call made the current one is put back."""
+    import rocmlir_amd.api as api
+    if api.torch is None:
+        api._load_torch()
+    entered = []
+
+    class Device:
+        def __init__(self, device):
+            pass
+
+        def __enter__(self):
+            entered.append(1)
+
+        def __exit__(self, *what):
+            entered.append(-1)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for bad in ("a stream", object()):
+        with pytest.raises((rock.RockError, TypeError, ValueError)):
+            api._on("test", torch.device("cuda", 0), bad)
+    assert entered == [1, -1, 1, -1]
