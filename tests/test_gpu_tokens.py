@@ -632,3 +632,40 @@ def test_whole_rounds_of_tiles_and_then_parts(rock, gpu, sizes, n, k, which, tra
             want = torch.zeros((n, k), dtype=torch.float64, device=gpu)
             want[some_n[:, None], some_k] = de.t() @ xe
             assert torch.equal(dw[e], (want if transB else want.t()).to(kind)), e
+
+
+@pytest.mark.parametrize("tile", TILES)
+@pytest.mark.parametrize("n,k", [(72, 80), (69, 77)], ids=["chunks", "any"])
+@pytest.mark.parametrize("transB", [True, False], ids=["NK", "KN"])
+@pytest.mark.parametrize("t", FLOATS)
+def test_what_is_not_finite_stays_in_its_row_and_column(rock, gpu, t, transB, n, k, tile):
+    """A NaN in a row of x, an infinity in a column of one expert's weights: what the 64-bit products hold, nothing in the
+    rows and experts beside them, in the product and in both gradients."""
+    sizes, tail = [30, 0, 70, 1], 2
+    g, T, E, x, w, dout, off = grouped_operands((sizes, tail, n, k), t, True, True, 23)
+    x[5, k - 1], w[2, n - 1, 3], dout[40, 2], x[29, 0] = float("nan"), float("inf"), float("inf"), float("-inf")
+    wd = (w if transB else w.transpose(1, 2).contiguous()).to(gpu)
+    xd, dd, offd, kw = x.to(gpu), dout.to(gpu), off.to(gpu), dict(transB=transB, perf_config="v2:" + tile)
+    y, dx = rock.grouped_gemm(xd, wd, offd, **kw).cpu(), rock.grouped_gemm_bwd_data(dd, wd, offd, **kw).cpu()
+    dw = rock.grouped_gemm_bwd_weight(xd, dd, offd, **kw).cpu()
+    same = lambda got, want: torch.equal(got.double().nan_to_num(nan=9e9), want.to(TORCH[t]).double().nan_to_num(nan=9e9))   # noqa: E731
+    for e, a, b in spans(sizes):
+        x64, d64, w64 = x[a:b].double(), dout[a:b].double(), w[e].double()
+        assert same(y[a:b], x64 @ w64.t()) and same(dx[a:b], d64 @ w64), e
+        assert same(dw[e], d64.t() @ x64 if transB else x64.t() @ d64), e
+
+
+@pytest.mark.parametrize("out", FLOATS)
+@pytest.mark.parametrize("rows,k", [(3, 256), (40, 256), (40, 77), (600, 256)])
+def test_poisoned_tokens_in_every_result_type(rock, gpu, out, rows, k):
+    g = generator(51)
+    x = torch.randn((rows, k), generator=g).to(torch.bfloat16)
+    x[rows // 2, 1] = float("inf")
+    w = whole(g, -127, 127, 96, k).to(torch.int8)
+    q, s = rock.quantize_tokens(x.to(gpu))
+    for trans in (True, False):
+        wd = (w if trans else w.t().contiguous()).to(gpu)
+        for y in (rock.gemm(q, wd, transB=trans, token_scale=s, out_dtype=out, relu=True),
+                  rock.grouped_gemm(q, wd[None], make_offsets([rows]).to(gpu), transB=trans, token_scale=s, out_dtype=out)):
+            bad = torch.arange(rows, device=gpu) == rows // 2
+            assert y[bad].isnan().all() and y[~bad].isfinite().all()
