@@ -89,7 +89,7 @@ const TokenTile *pick_token_tile(int64_t rows, int64_t groups, int64_t cols, con
 
 // The tile of a weight gradient: `groups` results of M x N, each the sum over about `depth` rows.  The large tile pays
 // where the reduction is long (8 experts 4096 x 2048 bf16, us: 2048 rows each 242 against 294 on 128 x 128 and 566 on
-// 64 x 64; 256 rows 60 / 58 / 85), short ones are bound by their results and the latency of each tile, which the four
+// 64 x 64; 256 rows 60 / 58 / 85), short ones are bound by their results and the latency of each tile, which the three
 // resident blocks of the 128 x 128 kernel hide (60 experts 1408 x 2048 at 83 rows 98 / 92 / 139; 64 experts 768 x 1024 at
 // 16 rows 30 / 23 / 33); few tiles want to be small (4 experts 512 x 512 at 1000 rows 15 / 18 / 14).  f32 results
 // stage in twice the LDS and the 128 x 128 kernel has two blocks (8 experts 1024 x 1024 at 250 rows 60 / 49 / 45).
