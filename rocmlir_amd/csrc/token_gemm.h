@@ -353,9 +353,9 @@ __device__ __forceinline__ void token_gemm_body_dl(const void *A, const void *B,
 // Rows shorter than a chunk are loaded element by element.
 // Measured on MI355X: int8 1001 x 2307 x 1283 19 us (1280 deep on the aligned 64 x 64 tiles 13, 1284 deep here 15, so four of
 // the six are the loads' alignment), 4000 x 4096 x 2051 on 128 x 128 tiles 94.  Rows of 1410 f16 start on 4-byte boundaries
-// and lose elsewhere: with three K-steps in registers a 128 x 128 wave takes 318 of them (190 and 128 accumulation registers) and its block a
-// unit to itself, where the aligned weight gradient runs three a unit.  60 groups 1410 x 2048 at 5003 rows: gradient of the rows 118 us, of the
-// weights 235 (1408 columns on the aligned kernels: 97 and 99).
+// and lose elsewhere: with three K-steps in registers a 128 x 128 wave takes 318 of them (190 and 128 accumulation
+// registers) and its block a unit to itself, where the aligned weight gradient runs three a unit.  60 groups 1410 x 2048 at
+// 5003 rows: gradient of the rows 118 us, of the weights 235 (1408 columns on the aligned kernels: 97 and 99).
 __device__ __forceinline__ v4i move_down(const v4i &v, int bytes) { // byte i <- byte i + bytes, zeros from behind
   typedef uint64_t v2u __attribute__((ext_vector_type(2)));
   const v2u w = __builtin_bit_cast(v2u, v);
